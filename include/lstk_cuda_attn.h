@@ -68,7 +68,7 @@ int lstk_cuda_status(void *stream);
  * in the device status, lets its in-flight copies and tensor-core work finish, frees its tensor
  * memory and returns, so the context stays usable. This sets, for later decode / prefill launches
  * from the calling host thread (lstk_cuda_attn_decode, _decode_partial, _decode_static,
- * _prefill):
+ * _decode_window, _decode_weights, _prefill and their forms):
  *   pipeline_wait_ns  limit of each wait between the kernels' own warps (0 = the default, 4 s);
  *                     the waits that drain in-flight work before a kernel exits keep 4 s;
  *   start_flag        optional device int32: the kernels' loaders wait (bounded by
@@ -162,6 +162,56 @@ int lstk_cuda_attn_decode_static(const lstk_kv_layout *layout, const void *k_cac
                                  const int32_t *block_tables, int32_t max_blocks_per_seq, const int32_t *seq_lens,
                                  int32_t max_seq_len, float scale, float *out, float *lse_out, int32_t n_ctas,
                                  void *stream);
+
+/* ---- Decode over a sliding window with sinks (no counterpart in the reference) ---------------
+ * lstk_cuda_attn_decode for a model or service that bounds its attention: the query of sequence b,
+ * at position n - 1 (n = seq_lens[b]), attends to its keys i >= n - window (the window holds its own
+ * key) and to the sinks i < n_sink. window >= 1, n_sink >= 0; either may exceed the sequence. Only the
+ * pages that hold visible keys are read: entries of block_tables between the sinks' last page and
+ * the window's first are not looked at, so the host may have reused those pages. Arguments, results,
+ * workspace and limits as lstk_cuda_attn_decode, except: out is f32 or bf16 (out_dtype; bf16, the input
+ * type of lstk_cuda_proj, rounds each f32 result once), and lse_out covers the visible keys.
+ * max_seq_len bounds seq_lens as there (it sizes the launch only). The _q8 form reads a q8_0 cache
+ * with lstk_cuda_attn_decode_q8's semantics, the query's block scale taken as amax * (1 / 127) in f32
+ * (a product: its last bit may differ from the quotient's there). */
+int lstk_cuda_attn_decode_window(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
+                                 int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                 int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len,
+                                 int32_t window, int32_t n_sink, float scale, void *out, int32_t out_dtype,
+                                 float *lse_out, void *workspace, size_t workspace_bytes, int32_t n_ctas, void *stream);
+int lstk_cuda_attn_decode_window_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d,
+                                    const int8_t *v_qs, const void *v_d, const void *q, int32_t q_dtype,
+                                    int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                    int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len,
+                                    int32_t window, int32_t n_sink, float scale, void *out, int32_t out_dtype,
+                                    float *lse_out, void *workspace, size_t workspace_bytes, int32_t n_ctas,
+                                    void *stream);
+
+/* ---- Decode that accumulates each key's attention weight (no counterpart in the reference) ----
+ * lstk_cuda_attn_decode, and for every visible key i of sequence b
+ *     acc[b * acc_stride + i] += sum over the query heads h of exp(scale * q_h k_i - lse_h)
+ * in f32, the heads in a fixed order (the same inputs and n_ctas give the same bits). Other entries of
+ * acc are left as they are, and an empty sequence's row is not touched. What acc holds decides which
+ * keys lstk_cuda_kv_evict_select keeps. out is f32 or bf16 as in lstk_cuda_attn_decode_window. Rows of
+ * acc hold at least max_seq_len keys (0 = max_blocks * block_size), and so does the workspace
+ * (lstk_cuda_attn_decode_weights_workspace_size, which includes the scores of the step: n_head * 4
+ * bytes per key); a sequence longer than max_seq_len reports LSTK_ERR_DEVICE_INDEX and attends to its
+ * first max_seq_len keys only. A key whose page id is out of range has no weight. The _q8 form as
+ * lstk_cuda_attn_decode_window_q8. */
+size_t lstk_cuda_attn_decode_weights_workspace_size(int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                                                    int32_t max_seq_len);
+int lstk_cuda_attn_decode_weights(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
+                                  int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                  int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len, float scale,
+                                  float *acc, int64_t acc_stride, void *out, int32_t out_dtype, float *lse_out,
+                                  void *workspace, size_t workspace_bytes, int32_t n_ctas, void *stream);
+int lstk_cuda_attn_decode_weights_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d,
+                                     const int8_t *v_qs, const void *v_d, const void *q, int32_t q_dtype,
+                                     int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                     int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len,
+                                     float scale, float *acc, int64_t acc_stride, void *out, int32_t out_dtype,
+                                     float *lse_out, void *workspace, size_t workspace_bytes, int32_t n_ctas,
+                                     void *stream);
 
 /* ---- Log-sum-exp merge of partial results over disjoint key ranges --------------------------
  * Used when one long context is split across GPUs (each GPU runs lstk_cuda_attn_decode over its

@@ -99,6 +99,16 @@ def lib():
                                         _I32, _P]
     L.lstk_cuda_attn_decode_partial.argtypes = [_P, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32, _I32,
                                                 ctypes.c_float, _P, _P, _P, _SZ, _I32, _P]
+    L.lstk_cuda_attn_decode_window.argtypes = [_LP, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32, _I32, _F,
+                                               _P, _I32, _P, _P, _SZ, _I32, _P]
+    L.lstk_cuda_attn_decode_window_q8.argtypes = [_LP, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _I32, _I32,
+                                                  _I32, _F, _P, _I32, _P, _P, _SZ, _I32, _P]
+    L.lstk_cuda_attn_decode_weights_workspace_size.argtypes = [_I32, _I32, _I32, _I32, _I32]
+    L.lstk_cuda_attn_decode_weights_workspace_size.restype = _SZ
+    L.lstk_cuda_attn_decode_weights.argtypes = [_LP, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _I32, _F, _P, _I64,
+                                                _P, _I32, _P, _P, _SZ, _I32, _P]
+    L.lstk_cuda_attn_decode_weights_q8.argtypes = [_LP, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _I32, _F,
+                                                   _P, _I64, _P, _I32, _P, _P, _SZ, _I32, _P]
     L.lstk_cuda_attn_merge.argtypes = [_P, _P, _I32, _I64, _I32, _I64, _I64, _P, _P, _P]
     L.lstk_cuda_kv_append_q8.argtypes = [_LP, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P, _P,
                                          _P, _P, _F, _P, _I32, _P, _I32, _P]

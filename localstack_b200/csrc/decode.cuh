@@ -23,6 +23,16 @@
 // 8-wide N side holds the GQA group (n_head / n_head_kv <= 8 query heads share one K/V head), so
 // every K/V byte brought in is used by all its query heads. The tensor cores only matter here
 // because they take the FLOPs off the issue slots; the kernel is bound by HBM bytes.
+//
+// Modes (kMode of the split kernel). kPlain: every key of the call's range. kWindow: keys
+// i >= len - window or i < n_sink; only the pages that hold such keys are streamed: a segment's
+// page-groups are its sink pages followed by its window pages (SeqPages), and keys outside both are
+// masked inside those pages (a 32-bit visibility mask per page). kWeights: kPlain, and every visible
+// score scale * q.k (log2 units, f32) also goes to a record of 32 keys per page-group and query row;
+// after the combine has the rows' log-sum-exps, weights_accumulate_kernel adds each key's softmax
+// weights, summed over the query heads, to a row of accumulated weights. The records cost
+// n_head * 8 bytes per key (written and read back, mostly from L2) next to the n_head_kv * 512 of K
+// and V; reading K again instead would cost n_head_kv * 256 and the dot products a second time.
 #pragma once
 
 #include <type_traits>
@@ -47,6 +57,8 @@ constexpr int kMaxGroup = 8;
 constexpr int kMaxSeqs = 4096;
 constexpr int kPartRows = kHeadsPerGroup * kMaxGroup;                // partial rows per piece
 
+enum Mode : int { kPlain = 0, kWindow = 1, kWeights = 2 };
+
 struct Params {
     const void *q;
     int q_f16;
@@ -67,6 +79,10 @@ struct Params {
     int q8_dpitch;              // q8_0 cache: bytes per cell row of a stage's scale tile (16 or 32)
     uint64_t wait_ns;           // limit of each pipeline wait (drains keep kWaitLimitNs)
     const int32_t *start_flag;  // optional: the producer waits for it to be non-zero before loading
+    int out_bf16 = 0;               // kWindow, kWeights: out is bf16 (each value rounded once), not f32
+    int window = 0, n_sink = 0;     // kWindow
+    float *scores = nullptr;        // kWeights: [page-group][score_rows][32]
+    int score_rows = 0;             // query rows of a full head group (KV heads x group)
 };
 
 // First page-group of CTA c's range: floor(c P / G). Computed in double precision, which is
@@ -83,6 +99,42 @@ __host__ __device__ inline int64_t range_lo(int c, int64_t P, int G) {
 __device__ __forceinline__ int range_len(const Params &p, int32_t len) {
     len = len < 0 ? 0 : min(len, p.max_blocks * kPage);
     return max(0, min(len, p.kv_end) - p.kv_page0 * kPage);
+}
+
+// The pages of a sequence that its query sees. Page-group p of a segment is page p (kPlain,
+// kWeights), or page p of the sinks' pages followed by the window's (kWindow): the sinks end in page
+// n_sink_pages - 1 at the latest, the window begins in page first_page; a page that holds both counts
+// as the window's.
+struct SeqPages {
+    int len;           // keys inside the call's range
+    int first;         // kWindow: the window's first key
+    int n_sink_pages;  // kWindow: pages before the gap
+    int skip;          // kWindow: pages inside the gap
+    __device__ __forceinline__ int page(int p) const { return p < n_sink_pages ? p : p + skip; }
+    __device__ __forceinline__ int count() const { return (len + kPage - 1) / kPage - skip; }
+    // Visible keys of page pg, bit i for its key i.
+    __device__ __forceinline__ uint32_t mask(int pg, int n_sink) const {
+        auto below = [&](int n) {  // keys of the page at positions < n
+            const int r = n - pg * kPage;
+            return r <= 0 ? 0u : r >= kPage ? 0xffffffffu : (1u << r) - 1u;
+        };
+        return below(len) & (~below(first) | below(n_sink));
+    }
+};
+
+template <int kMode>
+__device__ __forceinline__ SeqPages seq_pages(const Params &p, int32_t raw_len) {
+    SeqPages s;
+    s.len = range_len(p, raw_len);
+    s.first = s.n_sink_pages = s.skip = 0;
+    if constexpr (kMode == kWindow) {
+        s.first = max(0, s.len - p.window);
+        const int first_page = s.first / kPage;
+        // an empty sequence has first 0, so no sink pages
+        s.n_sink_pages = min((min(p.n_sink, s.first) + kPage - 1) / kPage, first_page);
+        s.skip = first_page - s.n_sink_pages;
+    }
+    return s;
 }
 
 // Index of the CTA whose range [lo_c, lo_{c+1}) contains page-group x.
@@ -190,14 +242,45 @@ __device__ __forceinline__ void load_q(HeadState &st, const Params &p, int b, in
     }
 }
 
-// One page (32 tokens, `valid` of them visible) of one KV head.
-__device__ __forceinline__ void process_page(HeadState &st, uint32_t kbase, uint32_t vbase, int valid,
-                                             float scale_log2, int lane) {
+// What of a page is visible: its first `valid` tokens (kPlain, kWeights) or the tokens of `mask`
+// (kWindow).
+template <int kMode>
+struct PageView {
+    int valid;
+    uint32_t mask;
+    __device__ __forceinline__ bool sees(int tok) const {
+        return kMode == kWindow ? ((mask >> tok) & 1u) != 0 : tok < valid;
+    }
+    __device__ __forceinline__ bool slab_empty(int slab) const {
+        return kMode == kWindow ? ((mask >> (16 * slab)) & 0xffffu) == 0 : slab * 16 >= valid;
+    }
+    __device__ __forceinline__ bool slab_partial(int slab) const {
+        return kMode == kWindow ? ((mask >> (16 * slab)) & 0xffffu) != 0xffffu : (slab + 1) * 16 > valid;
+    }
+};
+
+// kWeights: stores the scores x (tokens tok0, tok0 + 8 of query heads 2t, 2t + 1 of the KV head whose
+// record rows start at rec) of the visible tokens.
+__device__ __forceinline__ void store_scores(float *rec, int group, int t, int tok0, bool v0, bool v1, const float x[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (2 * t + h < group) {
+            float *row = rec + (2 * t + h) * kPage + tok0;
+            if (v0) row[0] = x[h];
+            if (v1) row[8] = x[h + 2];
+        }
+    }
+}
+
+// One page (32 tokens, those of `view` visible) of one KV head.
+template <int kMode>
+__device__ __forceinline__ void process_page(HeadState &st, uint32_t kbase, uint32_t vbase, const PageView<kMode> view,
+                                             float scale_log2, int lane, float *rec, int group) {
     const int g = lane >> 2, t = lane & 3;
     const int li = lane >> 3, lr = lane & 7;
 #pragma unroll
     for (int slab = 0; slab < 2; slab++) {
-        if (slab * 16 >= valid) break;
+        if (view.slab_empty(slab)) continue;
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < 8; kk++) {
@@ -207,12 +290,13 @@ __device__ __forceinline__ void process_page(HeadState &st, uint32_t kbase, uint
         }
         // s[0],s[1]: token slab*16+g, heads 2t,2t+1; s[2],s[3]: token +8.
         const int tok0 = slab * 16 + g;
-        const bool v0 = tok0 < valid, v1 = tok0 + 8 < valid;
+        const bool v0 = view.sees(tok0), v1 = view.sees(tok0 + 8);
         float x[4];
         x[0] = v0 ? s[0] * scale_log2 : -INFINITY;
         x[1] = v0 ? s[1] * scale_log2 : -INFINITY;
         x[2] = v1 ? s[2] * scale_log2 : -INFINITY;
         x[3] = v1 ? s[3] * scale_log2 : -INFINITY;
+        if constexpr (kMode == kWeights) store_scores(rec, group, t, tok0, v0, v1, x);
         float alpha[2], mu[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -238,7 +322,7 @@ __device__ __forceinline__ void process_page(HeadState &st, uint32_t kbase, uint
         }
         const uint32_t pb0 = movmatrix_trans(pack_half2(p0, p1));
         const uint32_t pb1 = movmatrix_trans(pack_half2(p2, p3));
-        const bool tail = (slab + 1) * 16 > valid;
+        const bool tail = view.slab_partial(slab);
 #pragma unroll
         for (int mt = 0; mt < 8; mt++) {
             uint32_t a[4];
@@ -247,8 +331,8 @@ __device__ __forceinline__ void process_page(HeadState &st, uint32_t kbase, uint
                 // Zero V where the token is not visible, so stale non-finite cells cannot leak
                 // through a zero probability. a0,a1: tokens 2t,2t+1; a2,a3: tokens 2t+8,2t+9.
                 const int tb = slab * 16 + 2 * t;
-                const uint32_t lo_keep = (tb < valid ? 0x0000ffffu : 0u) | (tb + 1 < valid ? 0xffff0000u : 0u);
-                const uint32_t hi_keep = (tb + 8 < valid ? 0x0000ffffu : 0u) | (tb + 9 < valid ? 0xffff0000u : 0u);
+                const uint32_t lo_keep = (view.sees(tb) ? 0x0000ffffu : 0u) | (view.sees(tb + 1) ? 0xffff0000u : 0u);
+                const uint32_t hi_keep = (view.sees(tb + 8) ? 0x0000ffffu : 0u) | (view.sees(tb + 9) ? 0xffff0000u : 0u);
                 a[0] &= lo_keep;
                 a[1] &= lo_keep;
                 a[2] &= hi_keep;
@@ -320,7 +404,10 @@ struct HeadStateQ8 {
 // Quantises query head g's row to q8_0 as ggml does for a q8_0 K (quantize_row_q8_0 of the f32
 // row: per 32 values d = amax / 127, q = round-to-nearest-even(x / d)), lane (g, t) keeping the
 // bytes its B fragments need (dims 32b + 4t.. and 32b + 16 + 4t..) and the four lanes of a head
-// reducing the block's amax; then gathers the scales of heads 2t, 2t + 1 (the S layout).
+// reducing the block's amax; then gathers the scales of heads 2t, 2t + 1 (the S layout). kWindow and
+// kWeights take d = amax * (1 / 127) in f32, a product in place of the quotient: d may differ from
+// kPlain's in its last bit.
+template <int kMode>
 __device__ __forceinline__ void load_q_q8(HeadStateQ8 &st, const Params &p, int b, int kvh, int lane) {
     const int g = lane >> 2, t = lane & 3;
     const bool live = g < p.group;
@@ -349,7 +436,7 @@ __device__ __forceinline__ void load_q_q8(HeadStateQ8 &st, const Params &p, int 
         for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const float d = __fdiv_rn(amax, 127.0f);
+        const float d = kMode == kPlain ? __fdiv_rn(amax, 127.0f) : __fmul_rn(amax, 1.0f / 127.0f);
         const float id = d != 0.f ? __frcp_rn(d) : 0.f;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -380,19 +467,21 @@ __device__ __forceinline__ void i8x4_to_f16x2x2(uint32_t r, uint32_t &even, uint
     odd = *reinterpret_cast<const uint32_t *>(&o);
 }
 
-// One page (32 tokens, `valid` visible) of one KV head over the q8_0 planes. S: per 32-dim block
+// One page (32 tokens, those of `view` visible) of one KV head over the q8_0 planes. S: per 32-dim block
 // an int8 MMA (m16n8k32) gives the exact integer dot of the K and Q blocks; the score is
 // sum_b (d_k,b * d_q,b) * dot_b in block order, as ggml's q8_0 x q8_0 dot. PV: V's int8 values
 // become f16 exactly and each block's scale d_v multiplies P instead (P' = P * d_v per key and
 // block, rounded to f16 like P itself), so O^T += V^T . P'^T per 16-dim m-tile; the tile's rows
 // are dims 2g, 2g + 1 of its 16 (the pairs ldmatrix.trans delivers).
+template <int kMode>
 __device__ __forceinline__ void process_page_q8(HeadStateQ8 &st, uint32_t kbase, uint32_t vbase, const uint8_t *kd,
-                                                const uint8_t *vd, int dpitch, int valid, float scale_log2, int lane,
-                                                int slab_lo, int slab_hi) {
+                                                const uint8_t *vd, int dpitch, const PageView<kMode> view,
+                                                float scale_log2, int lane, int slab_lo, int slab_hi, float *rec,
+                                                int group) {
     const int g = lane >> 2, t = lane & 3;
     const int li = lane >> 3, lr = lane & 7;
     for (int slab = slab_lo; slab < slab_hi; slab++) {
-        if (slab * 16 >= valid) break;
+        if (view.slab_empty(slab)) continue;
         const int tok0 = slab * 16 + g;
         int sb[4][4];
 #pragma unroll
@@ -426,12 +515,13 @@ __device__ __forceinline__ void process_page_q8(HeadStateQ8 &st, uint32_t kbase,
                 acc = fmaf((float) sb[blk][i], dk[i >> 1][blk] * st.dq[i & 1][blk], acc);
             s[i] = acc;
         }
-        const bool v0 = tok0 < valid, v1 = tok0 + 8 < valid;
+        const bool v0 = view.sees(tok0), v1 = view.sees(tok0 + 8);
         float x[4];
         x[0] = v0 ? s[0] * scale_log2 : -INFINITY;
         x[1] = v0 ? s[1] * scale_log2 : -INFINITY;
         x[2] = v1 ? s[2] * scale_log2 : -INFINITY;
         x[3] = v1 ? s[3] * scale_log2 : -INFINITY;
+        if constexpr (kMode == kWeights) store_scores(rec, group, t, tok0, v0, v1, x);
         float alpha[2], mu[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -493,8 +583,8 @@ __device__ __forceinline__ void process_page_q8(HeadStateQ8 &st, uint32_t kbase,
 extern __shared__ __align__(1024) uint8_t dyn_smem[];
 
 // kQ8: the cache is q8_0 planes (kmap / vmap over the qs planes, kdmap / vdmap over the scale
-// planes); else f16 rows (kmap / vmap; the scale maps are unused).
-template <bool kQ8>
+// planes); else f16 rows (kmap / vmap; the scale maps are unused). kMode: see the top of this file.
+template <bool kQ8, int kMode = kPlain>
 __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_split_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                     const __grid_constant__ CUtensorMap vmap,
                                                                     const __grid_constant__ CUtensorMap kdmap,
@@ -547,7 +637,7 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
     if (warp >= 1 && warp < kConsumers) {
         const int t = threadIdx.x - 32;
         if (t * 32 < p.n_seqs) prefetch_l2(p.seq_lens + t * 32);
-        if (p.n_seqs == 1) {
+        if (kMode != kWindow && p.n_seqs == 1) {
             const int64_t span =
                 min((int64_t) p.max_blocks, ((int64_t) p.kv_end + kPage - 1) / kPage) - (int64_t) p.kv_page0;
             if (span > 0) {
@@ -577,8 +667,10 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
         int32_t local = 0;
         for (int b = b0; b < min(b0 + per, p.n_seqs); b++) {
             const int32_t len = p.seq_lens[b];
-            if (len < 0 || len > p.max_blocks * kPage) report(p.status, kStatusBadIndex, kSiteDecodeLen, b);
-            local += (range_len(p, len) + kPage - 1) / kPage;
+            // kWeights: the records and the weight rows hold kv_end keys, and no more are attended to
+            if (len < 0 || len > p.max_blocks * kPage || (kMode == kWeights && len > p.kv_end))
+                report(p.status, kStatusBadIndex, kSiteDecodeLen, b);
+            local += seq_pages<kMode>(p, len).count();
         }
         int32_t incl = local;
 #pragma unroll
@@ -592,7 +684,7 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
         for (int w = 0; w < warp; w++) acc += warp_tot[w];
         for (int b = b0; b < min(b0 + per, p.n_seqs); b++) {
             pfx[b] = acc;
-            acc += (range_len(p, p.seq_lens[b]) + kPage - 1) / kPage;
+            acc += seq_pages<kMode>(p, p.seq_lens[b]).count();
         }
         if (threadIdx.x == kNThreads - 1) pfx[p.n_seqs] = acc;
         __syncthreads();
@@ -630,7 +722,9 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
                 Cursor c;
                 c.locate(x, pfx, p.n_seqs, p.n_hg);
                 hg = c.hg;
-                pid = p.block_tables[(int64_t) c.b * p.max_blocks + p.kv_page0 + c.p];
+                int page = p.kv_page0 + c.p;
+                if constexpr (kMode == kWindow) page = seq_pages<kMode>(p, p.seq_lens[c.b]).page(c.p);
+                pid = p.block_tables[(int64_t) c.b * p.max_blocks + page];
             }
         };
         int32_t pid_next;
@@ -707,7 +801,7 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
         cur.locate(lo, pfx, p.n_seqs, p.n_hg);
         int64_t piece_start = lo;
         int64_t i = 0;
-        int len = 0;  // keys of the current segment's sequence inside the call's range
+        SeqPages sp = {0, 0, 0, 0};  // the current segment's sequence
         for (int64_t x = lo; x < hi; x++, i++) {
             const int np = pfx[cur.b + 1] - pfx[cur.b];
             const int kvh = cur.hg * kHeadsPerGroup + hw;
@@ -716,10 +810,10 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
                 piece_start = x;
                 st.reset();
                 if (active) {
-                    if constexpr (kQ8) load_q_q8(st, p, cur.b, kvh, lane);
+                    if constexpr (kQ8) load_q_q8<kMode>(st, p, cur.b, kvh, lane);
                     else load_q(st, p, cur.b, kvh, lane);
                 }
-                len = range_len(p, p.seq_lens[cur.b]);
+                sp = seq_pages<kMode>(p, p.seq_lens[cur.b]);
             }
             const int s = (int) (i % kNStages);
             // Warp-uniform outcome: ldmatrix / mma.sync below are warp-collective.
@@ -733,17 +827,26 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
             }
             const int32_t pid = stage_pid[s];
             if (active && pid >= 0 && pid < p.n_pages) {
-                const int valid = min(kPage, len - cur.p * kPage);
+                PageView<kMode> view;
+                float *rec = nullptr;
+                if constexpr (kMode == kWindow) view = {0, sp.mask(sp.page(cur.p), p.n_sink)};
+                else view = {min(kPage, sp.len - cur.p * kPage), 0u};
+                if constexpr (kMode == kWeights) rec = p.scores + (x * p.score_rows + hw * p.group) * kPage;
                 const uint32_t sb = smem_u32(stages + (size_t) s * kSBytes);
                 if constexpr (kQ8) {
                     const uint8_t *st_base = stages + (size_t) s * kSBytes;
                     process_page_q8(st, sb + hw * kQ8HeadPage, sb + kQ8VOff + hw * kQ8HeadPage,
-                                    st_base + kQ8KdOff + hw * 8, st_base + kQ8VdOff + hw * 8, p.q8_dpitch, valid,
-                                    p.scale_log2, lane, half, half + 1);
+                                    st_base + kQ8KdOff + hw * 8, st_base + kQ8VdOff + hw * 8, p.q8_dpitch, view,
+                                    p.scale_log2, lane, half, half + 1, rec, p.group);
                 } else {
                     process_page(st, sb + warp * kHeadPage, sb + kHeadsPerGroup * kHeadPage + warp * kHeadPage,
-                                 valid, p.scale_log2, lane);
+                                 view, p.scale_log2, lane, rec, p.group);
                 }
+            } else if constexpr (kMode == kWeights) {
+                // a page with a bad id (reported): its keys have no weight
+                if (active && half == 0)
+                    for (int r = 0; r < p.group; r++)
+                        p.scores[(x * p.score_rows + hw * p.group + r) * kPage + lane] = -INFINITY;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
@@ -817,6 +920,22 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
                         const float inv = l[h] > 0.f ? 1.f / l[h] : 0.f;
                         const float lse2 = l[h] > 0.f ? st.m[h] + __log2f(l[h]) : -INFINITY;
                         float *dst;
+                        if (kMode != kPlain && whole && p.out_bf16) {
+                            const int64_t row = (int64_t) cur.b * p.n_head + (int64_t) kvh * p.group + n;
+                            if (g == 0 && p.lse_out != nullptr) p.lse_out[row] = lse2 * 0.69314718055994531f;
+                            __nv_bfloat16 *d16 = reinterpret_cast<__nv_bfloat16 *>(p.out) + row * kD;
+#pragma unroll
+                            for (int mt = 0; mt < 8; mt++) {
+                                const float a = st.o[mt][h] * inv, c = st.o[mt][h + 2] * inv;
+                                if constexpr (kQ8) {
+                                    *reinterpret_cast<__nv_bfloat162 *>(d16 + mt * 16 + 2 * g) = __floats2bfloat162_rn(a, c);
+                                } else {
+                                    d16[mt * 16 + g] = __float2bfloat16_rn(a);
+                                    d16[mt * 16 + g + 8] = __float2bfloat16_rn(c);
+                                }
+                            }
+                            continue;
+                        }
                         if (whole) {
                             dst = p.out + ((int64_t) cur.b * p.n_head + (int64_t) kvh * p.group + n) * kD;
                             if (g == 0 && p.lse_out != nullptr)
@@ -858,6 +977,7 @@ struct CombineParams {
     const float *part_lse;
     float *out;
     float *lse_out;
+    int out_bf16;  // out is bf16 (the kernels instantiated for a typed output only)
     // Exchange across ranks (decode_combine_kernel<true>): the mailboxes of the exchange-merge
     // protocol (exchange.cuh) for n_seqs * n_head rows, this rank, the rank count, the flag-wait
     // bound and the device status.
@@ -927,13 +1047,18 @@ struct ExchangeState {
 // call by every CTA of the grid (see advance_epoch), so calls replay from a CUDA graph and the
 // CTAs of one row always agree on it; words alternate between two banks by epoch parity (a rank
 // is at most one call ahead of a peer: it needs the peer's row of the current call to finish it).
-template <bool kExchange>
+template <bool kExchange, bool kTyped>
 __device__ __forceinline__ void finish_row(const CombineParams &p, int64_t row, int d0, int nd, float o, float lse,
                                            const ExchangeState &xs) {
     const int tid = threadIdx.x;
     const bool first = d0 == 0;
     if constexpr (!kExchange) {
-        if (tid < nd) p.out[row * kD + d0 + tid] = o;
+        if (tid < nd) {
+            if (kTyped && p.out_bf16)
+                reinterpret_cast<__nv_bfloat16 *>(p.out)[row * kD + d0 + tid] = __float2bfloat16_rn(o);
+            else
+                p.out[row * kD + d0 + tid] = o;
+        }
         if (tid == 0 && first && p.lse_out != nullptr) p.lse_out[row] = lse;
     } else {
         // Thread t < nd sends its dim's word to every peer and polls the same dim's word of every
@@ -1043,7 +1168,7 @@ __device__ __forceinline__ void merge_state(float &m, float &den, float4 &acc, f
 // (max, sum, accumulator) state, merged across lane groups by shuffles and across warps in shared
 // memory. Piece i is split CTA c0 + i; its record is slot 0 of that CTA's pair, except for the
 // first piece when the CTA's range began in an earlier segment (slot 1).
-template <bool kExchange>
+template <bool kExchange, bool kTyped = false>
 __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(const CombineParams p) {
     pdl_wait();  // the split grid's partials and prefix are complete and visible
     const int S = p.dsplit;
@@ -1197,7 +1322,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
         o = total > 0.f ? o / total : 0.f;
         row_lse = total > 0.f ? (M + __log2f(total)) * 0.69314718055994531f : -INFINITY;
     }
-    finish_row<kExchange>(p, out_row, d0, nd, o, row_lse, xs);
+    finish_row<kExchange, kTyped>(p, out_row, d0, nd, o, row_lse, xs);
     advance_epoch<kExchange>(p, xs);
 }
 
@@ -1207,6 +1332,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
 // and writing the row, so nothing crosses warps after the segment's plan, which thread 0 works
 // out once for the CTA's eight rows. Chosen where segments have few pieces (many sequences per
 // grid); a long row over many pieces takes decode_combine_kernel, which spreads it over CTAs.
+template <bool kTyped>
 __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_rows_kernel(const CombineParams p) {
     pdl_wait();  // the split grid's partials and prefix are complete and visible
     const int b = blockIdx.x, hg = blockIdx.y, w = blockIdx.z;
@@ -1235,9 +1361,17 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_rows_kernel
     const int mode = plan_s[0];
     if (n >= p.group || mode == 2) return;
     const int64_t out_row = (int64_t) b * p.n_head + (int64_t) kvh * p.group + n;
-    float4 *dst = reinterpret_cast<float4 *>(p.out + out_row * kD) + lane;
+    auto store = [&](const float4 v) {
+        if (kTyped && p.out_bf16) {
+            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+            reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + out_row * kD)[lane] =
+                *reinterpret_cast<const uint2 *>(h);
+        } else {
+            reinterpret_cast<float4 *>(p.out + out_row * kD)[lane] = v;
+        }
+    };
     if (mode == 1) {
-        *dst = make_float4(0.f, 0.f, 0.f, 0.f);
+        store(make_float4(0.f, 0.f, 0.f, 0.f));
         if (lane == 0 && p.lse_out != nullptr) p.lse_out[out_row] = -INFINITY;
         return;
     }
@@ -1280,9 +1414,59 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_rows_kernel
     }
     // Divided as decode_combine_kernel divides: a row of up to 8 pieces then gets the same bits
     // from both kernels (the same weights, summed in piece order).
-    *dst = den > 0.f ? make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den) : make_float4(0.f, 0.f, 0.f, 0.f);
+    store(den > 0.f ? make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den) : make_float4(0.f, 0.f, 0.f, 0.f));
     if (lane == 0 && p.lse_out != nullptr)
         p.lse_out[out_row] = den > 0.f ? (m + __log2f(den)) * 0.69314718055994531f : -INFINITY;
+}
+
+// kWeights, after the combine: acc[b][i] += sum over the query rows r of 2^(score[r][i] - lse2[r]), the
+// softmax weights of key i, with the rows in a fixed order and one thread per key (no atomics: the
+// same inputs give the same bits). A warp takes one page - lane i its key i - and reads that page's
+// record rows of 128 bytes. Rows without a finite maximum (no keys, or every score -inf) add nothing.
+struct AccumulateParams {
+    int n_seqs, n_head, n_head_kv, group, n_hg, score_rows;
+    int max_len;  // keys a row may hold (the split kernel's kv_end and table bound)
+    const int32_t *prefix;
+    const int32_t *seq_lens;
+    const float *scores;
+    const float *lse;  // [n_seqs][n_head], natural log
+    float *acc;
+    int64_t acc_stride;
+};
+
+constexpr int kAccumulateThreads = 256;
+
+__global__ void __launch_bounds__(kAccumulateThreads) weights_accumulate_kernel(const AccumulateParams p) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int n_pages = p.prefix[p.n_seqs];
+    for (int y = blockIdx.x * (kAccumulateThreads / 32) + (threadIdx.x >> 5); y < n_pages;
+         y += gridDim.x * (kAccumulateThreads / 32)) {
+        int lo = 0, hi = p.n_seqs;  // largest b with prefix[b] <= y: the sequence that holds page y
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (p.prefix[mid] <= y) lo = mid; else hi = mid - 1;
+        }
+        const int b = lo, pb = p.prefix[b], np = p.prefix[b + 1] - pb, pg = y - pb;
+        const int len = min(max(p.seq_lens[b], 0), p.max_len);
+        const bool live = pg * kPage + lane < len;
+        float w = 0.f;
+        for (int hg = 0; hg < p.n_hg; hg++) {
+            const int rows = min(kHeadsPerGroup, p.n_head_kv - hg * kHeadsPerGroup) * p.group;
+            const int64_t x = (int64_t) p.n_hg * pb + (int64_t) hg * np + pg;
+            const float *rec = p.scores + x * p.score_rows * kPage + lane;
+            // lane r: lse (log2 units) of the group's row r; +inf makes an empty row's weights 0
+            const float l = lane < rows ? p.lse[(int64_t) b * p.n_head + (int64_t) hg * kHeadsPerGroup * p.group + lane]
+                                        : -INFINITY;
+            const float l2 = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
+#pragma unroll 8
+            for (int r = 0; r < rows; r++) {
+                const float lr = __shfl_sync(0xffffffffu, l2, r);
+                if (live) w += fast_exp2(rec[r * kPage] - lr);
+            }
+        }
+        if (live) p.acc[(int64_t) b * p.acc_stride + pg * kPage + lane] += w;
+    }
 }
 
 // LSE merge of n_parts partial results (natural-log lse), one warp per output row.

@@ -35,6 +35,7 @@ struct DeviceInfo {
     // Dynamic shared-memory limits raised so far on this device, per kernel (ensure_smem).
     size_t decode_smem = 0;
     size_t decode_q8_smem = 0;
+    size_t decode_mode_smem[2][3] = {};  // per [q8_0][mode] (windowed, with accumulated weights)
     size_t prefill_smem = 0;
     size_t append_smem[8] = {};  // per kv_append instantiation (append_kernel)
     size_t gemm_smem = 0;
@@ -440,10 +441,29 @@ struct ExchangeSpec {
     uint64_t wait_ns;
 };
 
+// A decode over a window with sinks, or one that accumulates the keys' weights (decode.cuh's modes).
+struct ModeSpec {
+    const char *fn;  // the entry point, for its messages
+    int mode;
+    int32_t out_dtype;
+    int32_t window, n_sink;  // decode::kWindow
+    float *acc;              // decode::kWeights
+    int64_t acc_stride;
+};
+
+typedef void (*SplitKernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, decode::Params);
+static SplitKernel split_kernel(bool q8, int mode) {
+    using namespace decode;
+    static const SplitKernel k[2][3] = {
+        {decode_split_kernel<false, kPlain>, decode_split_kernel<false, kWindow>, decode_split_kernel<false, kWeights>},
+        {decode_split_kernel<true, kPlain>, decode_split_kernel<true, kWindow>, decode_split_kernel<true, kWeights>}};
+    return k[q8 ? 1 : 0][mode];
+}
+
 // kdmap / vdmap: the scale-plane maps of a q8_0 cache (q8 true), else ignored.
 static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const CUtensorMap &kdmap,
                          const CUtensorMap &vdmap, bool q8, const decode::Params &p, int grid, size_t smem,
-                         int n_sms, cudaStream_t s, const ExchangeSpec *ex = nullptr) {
+                         int n_sms, cudaStream_t s, const ExchangeSpec *ex = nullptr, int mode = decode::kPlain) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -454,12 +474,8 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    int rc = q8 ? launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::decode_split_kernel<true>, kmap, vmap, kdmap,
-                                                      vdmap, p),
-                                   "decode_split_kernel (q8_0)")
-                : launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::decode_split_kernel<false>, kmap, vmap, kdmap,
-                                                      vdmap, p),
-                                   "decode_split_kernel");
+    int rc = launch_pdl_check(cudaLaunchKernelEx(&cfg, split_kernel(q8, mode), kmap, vmap, kdmap, vdmap, p),
+                              q8 ? "decode_split_kernel (q8_0)" : "decode_split_kernel");
     if (rc) return rc;
     decode::CombineParams c;
     c.n_seqs = p.n_seqs;
@@ -473,6 +489,7 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
     c.part_lse = p.part_lse;
     c.out = p.out;
     c.lse_out = p.lse_out;
+    c.out_bf16 = p.out_bf16;
     c.mailboxes = ex ? ex->mailboxes : nullptr;
     c.rank = ex ? ex->rank : 0;
     c.n_ranks = ex ? ex->n_ranks : 1;
@@ -483,14 +500,21 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
     cfg.dynamicSmemBytes = 0;
     if (!ex && decode::combine_by_rows(p.n_seqs, p.n_hg, grid)) {
         cfg.gridDim = dim3((unsigned) p.n_seqs, (unsigned) p.n_hg, decode::kHeadsPerGroup);
-        return launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::decode_combine_rows_kernel, c),
+        return launch_pdl_check(cudaLaunchKernelEx(&cfg,
+                                                   p.out_bf16 ? decode::decode_combine_rows_kernel<true>
+                                                              : decode::decode_combine_rows_kernel<false>,
+                                                   c),
                                 "decode_combine_rows_kernel");
     }
     cfg.gridDim = dim3((unsigned) p.n_seqs, (unsigned) p.n_hg, (unsigned) (decode::kPartRows * c.dsplit));
     if (ex)
         return launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::decode_combine_kernel<true>, c),
                                 "decode_combine_kernel (exchange)");
-    return launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::decode_combine_kernel<false>, c), "decode_combine_kernel");
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg,
+                                               p.out_bf16 ? decode::decode_combine_kernel<false, true>
+                                                          : decode::decode_combine_kernel<false, false>,
+                                               c),
+                            "decode_combine_kernel");
 }
 
 size_t lstk_cuda_attn_decode_workspace_size(int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t head_dim) {
@@ -501,37 +525,77 @@ size_t lstk_cuda_attn_decode_workspace_size(int32_t n_seqs, int32_t n_head, int3
     return decode_ws_prefix_bytes(n_seqs) + kDecodePartLseBytes + kDecodePartOBytes;
 }
 
+static int launch_pdl(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, cudaStream_t s);
+
+// Workspace of lstk_cuda_attn_decode_weights: [decode workspace][lse][score records], each 256-byte
+// aligned. A record holds 32 keys' scores of every query row of a head group, in f32.
+static size_t weights_ws_lse_bytes(int32_t n_seqs, int32_t n_head) {
+    return align_up(sizeof(float) * (size_t) n_seqs * n_head, 256);
+}
+static int weights_score_rows(int32_t n_head, int32_t n_head_kv) {
+    return std::min(n_head_kv, decode::kHeadsPerGroup) * (n_head / n_head_kv);
+}
+size_t lstk_cuda_attn_decode_weights_workspace_size(int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                                                    int32_t max_seq_len) {
+    if (n_seqs < 0 || n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || max_seq_len < 0) return 0;
+    const size_t n_hg = (n_head_kv + decode::kHeadsPerGroup - 1) / decode::kHeadsPerGroup;
+    const size_t pages = ((size_t) max_seq_len + decode::kPage - 1) / decode::kPage;
+    return align_up(lstk_cuda_attn_decode_workspace_size(n_seqs, n_head, n_head_kv, head_dim), 256) +
+           weights_ws_lse_bytes(n_seqs, n_head) +
+           (size_t) n_seqs * pages * n_hg * weights_score_rows(n_head, n_head_kv) * decode::kPage * sizeof(float);
+}
+
 static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
                         int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
                         int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len, int32_t kv_begin,
                         int32_t kv_end, float scale, float *out, float *lse_out, void *workspace,
                         size_t workspace_bytes, int32_t n_ctas, void *stream, const ExchangeSpec *ex = nullptr,
-                        const Q8Planes *q8 = nullptr) {
-    int rc = check_layout(layout, "lstk_cuda_attn_decode");
+                        const Q8Planes *q8 = nullptr, const ModeSpec *ms = nullptr) {
+    const char *fn = ms ? ms->fn : "lstk_cuda_attn_decode";
+    const int mode = ms ? ms->mode : decode::kPlain;
+    int rc = check_layout(layout, fn);
     if (rc) return rc;
+    if (ms) {
+        if (ms->out_dtype != LSTK_DTYPE_F32 && ms->out_dtype != LSTK_DTYPE_BF16)
+            return set_error(LSTK_ERR_UNSUPPORTED, std::string(fn) + ": out_dtype must be f32 or bf16");
+        if (max_blocks_per_seq > INT32_MAX / layout->block_size)
+            return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": max_blocks_per_seq out of range");
+        if (mode == decode::kWindow && (ms->window < 1 || ms->n_sink < 0))
+            return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": window must be at least 1 and n_sink at least 0");
+        if (mode == decode::kWeights && (!ms->acc || !aligned(ms->acc, 4)))
+            return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": acc is NULL or misaligned");
+    }
     const int hkv = layout->n_head_kv;
     if (n_seqs < 0 || n_head <= 0 || n_head % hkv != 0 || max_blocks_per_seq <= 0)
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_decode: bad n_seqs / n_head / max_blocks_per_seq");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad n_seqs / n_head / max_blocks_per_seq");
     const int group = n_head / hkv;
     if (group > decode::kMaxGroup)
-        return set_error(LSTK_ERR_UNSUPPORTED, "lstk_cuda_attn_decode: n_head / n_head_kv must be at most 8");
+        return set_error(LSTK_ERR_UNSUPPORTED, std::string(fn) + ": n_head / n_head_kv must be at most 8");
     if (n_seqs > decode::kMaxSeqs)
-        return set_error(LSTK_ERR_CAPACITY, "lstk_cuda_attn_decode: more than 4096 sequences in one call");
+        return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": more than 4096 sequences in one call");
     if (q_dtype != LSTK_DTYPE_F32 && q_dtype != LSTK_DTYPE_F16)
-        return set_error(LSTK_ERR_UNSUPPORTED, "lstk_cuda_attn_decode: q_dtype must be f32 or f16");
+        return set_error(LSTK_ERR_UNSUPPORTED, std::string(fn) + ": q_dtype must be f32 or f16");
     if (!k_cache || !v_cache || !q || !block_tables || !seq_lens || !out || !workspace)
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_decode: NULL pointer");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL pointer");
     if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(q, 16) || !aligned(out, 16) ||
         !aligned(workspace, 256))
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_decode: misaligned pointer");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": misaligned pointer");
     if (workspace_bytes < lstk_cuda_attn_decode_workspace_size(n_seqs, n_head, hkv, layout->head_dim))
-        return set_error(LSTK_ERR_CAPACITY, "lstk_cuda_attn_decode: workspace too small");
+        return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": workspace too small");
     if (max_seq_len <= 0 || max_seq_len > max_blocks_per_seq * layout->block_size)
         max_seq_len = max_blocks_per_seq * layout->block_size;
     if (kv_begin < 0 || kv_end < kv_begin || kv_begin % layout->block_size != 0 ||
         kv_begin > max_blocks_per_seq * layout->block_size)
         return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_decode_partial: kv_begin must be a page multiple <= kv_end");
     max_seq_len = std::max(0, std::min(max_seq_len, kv_end) - kv_begin);
+    if (mode == decode::kWeights) {
+        kv_end = max_seq_len;  // the records and the rows of acc hold this many keys of a sequence
+        if (ms->acc_stride < max_seq_len)
+            return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": a row of acc must hold max_seq_len keys");
+        if (workspace_bytes <
+            lstk_cuda_attn_decode_weights_workspace_size(n_seqs, n_head, hkv, layout->head_dim, max_seq_len))
+            return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": workspace too small");
+    }
     if (n_seqs == 0) return clear_error();
     DeviceInfo *dev = nullptr;
     if ((rc = bind_device(k_cache, &dev))) return rc;
@@ -540,9 +604,9 @@ static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const
     int dpitch = 0;
     if (q8) {
         if (hkv % 2 != 0)
-            return set_error(LSTK_ERR_UNSUPPORTED, "lstk_cuda_attn_decode_q8: n_head_kv must be even (16-byte scale rows)");
+            return set_error(LSTK_ERR_UNSUPPORTED, std::string(ms ? fn : "lstk_cuda_attn_decode_q8") + ": n_head_kv must be even (16-byte scale rows)");
         if (!aligned(q8->k_qs, 16) || !aligned(q8->v_qs, 16) || !aligned(q8->k_d, 16) || !aligned(q8->v_d, 16))
-            return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_decode_q8: planes must be 16-byte aligned");
+            return set_error(LSTK_ERR_INVALID_ARG, std::string(ms ? fn : "lstk_cuda_attn_decode_q8") + ": planes must be 16-byte aligned");
         dpitch = std::min(hkv, decode::kHeadsPerGroup) * 8;  // the scale tile's row: 4 f16 per head
         if ((rc = encode_3d(&kmap, q8->k_qs, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 128, hkv, layout->n_cells, 128, 1, 32)))
             return rc;
@@ -560,7 +624,11 @@ static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const
     }
 
     const int n_hg = (hkv + decode::kHeadsPerGroup - 1) / decode::kHeadsPerGroup;
-    const int64_t max_groups = (int64_t) n_seqs * n_hg * ((max_seq_len + decode::kPage - 1) / decode::kPage);
+    int64_t max_pages = (max_seq_len + decode::kPage - 1) / decode::kPage;
+    if (mode == decode::kWindow)  // the window may begin inside a page; the sinks begin at key 0
+        max_pages = std::min<int64_t>(max_pages, ((int64_t) ms->window + 2 * decode::kPage - 2) / decode::kPage +
+                                                     ((int64_t) ms->n_sink + decode::kPage - 1) / decode::kPage);
+    const int64_t max_groups = (int64_t) n_seqs * n_hg * max_pages;
     // q8_0: two CTAs per SM (a slab's dependent chain of int8 MMAs, scales and conversions needs
     // more warps per SM than the f16 kernel to keep HBM busy)
     int64_t grid = n_ctas > 0 ? n_ctas : (q8 ? 2 : 1) * dev->n_sms;
@@ -591,9 +659,23 @@ static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const
     p.wait_ns = t_pipeline_wait_ns;
     p.start_flag = t_start_flag;
     p.q8_dpitch = dpitch;
+    p.out_bf16 = ms && ms->out_dtype == LSTK_DTYPE_BF16;
+    p.window = ms ? ms->window : 0;
+    p.n_sink = ms ? ms->n_sink : 0;
+    p.scores = nullptr;
+    p.score_rows = weights_score_rows(n_head, hkv);
+    if (mode == decode::kWeights) {
+        uint8_t *more = ws + align_up(lstk_cuda_attn_decode_workspace_size(n_seqs, n_head, hkv, layout->head_dim), 256);
+        if (!lse_out) p.lse_out = reinterpret_cast<float *>(more);  // the accumulation needs it
+        p.scores = reinterpret_cast<float *>(more + weights_ws_lse_bytes(n_seqs, n_head));
+    }
 
     const size_t smem = q8 ? decode::split_smem_bytes<true>(n_seqs) : decode::split_smem_bytes<false>(n_seqs);
-    if (q8) {
+    if (ms) {
+        if ((rc = ensure_smem(&dev->decode_mode_smem[q8 ? 1 : 0][mode], split_kernel(q8 != nullptr, mode), smem,
+                              "cudaFuncSetAttribute(decode)")))
+            return rc;
+    } else if (q8) {
         if ((rc = ensure_smem(&dev->decode_q8_smem, decode::decode_split_kernel<true>, smem,
                               "cudaFuncSetAttribute(decode q8_0)")))
             return rc;
@@ -601,8 +683,31 @@ static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const
                                  "cudaFuncSetAttribute(decode)"))) {
         return rc;
     }
-    return launch_decode(kmap, vmap, kdmap, vdmap, q8 != nullptr, p, (int) grid, smem, dev->n_sms,
-                         static_cast<cudaStream_t>(stream), ex);
+    rc = launch_decode(kmap, vmap, kdmap, vdmap, q8 != nullptr, p, (int) grid, smem, dev->n_sms,
+                       static_cast<cudaStream_t>(stream), ex, mode);
+    if (rc || mode != decode::kWeights) return rc;
+    decode::AccumulateParams a;
+    a.n_seqs = n_seqs;
+    a.n_head = n_head;
+    a.n_head_kv = hkv;
+    a.group = group;
+    a.n_hg = n_hg;
+    a.score_rows = p.score_rows;
+    a.max_len = max_seq_len;
+    a.prefix = p.prefix;
+    a.seq_lens = seq_lens;
+    a.scores = p.scores;
+    a.lse = p.lse_out;
+    a.acc = ms->acc;
+    a.acc_stride = ms->acc_stride;
+    constexpr int kPagesPerCta = decode::kAccumulateThreads / 32;
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) std::max<int64_t>(
+        1, std::min<int64_t>((n_seqs * max_pages + kPagesPerCta - 1) / kPagesPerCta, (int64_t) dev->n_sms * 8)));
+    cfg.blockDim = dim3(decode::kAccumulateThreads);
+    launch_pdl(cfg, attr, static_cast<cudaStream_t>(stream));
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::weights_accumulate_kernel, a), "weights_accumulate_kernel");
 }
 
 int lstk_cuda_attn_decode(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
@@ -662,7 +767,61 @@ int lstk_cuda_attn_decode_q8(const lstk_kv_layout *layout, const int8_t *k_qs, c
                         nullptr, &q8);
 }
 
-static int launch_pdl(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, cudaStream_t s);
+int lstk_cuda_attn_decode_window(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
+                                 int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                 int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len,
+                                 int32_t window, int32_t n_sink, float scale, void *out, int32_t out_dtype,
+                                 float *lse_out, void *workspace, size_t workspace_bytes, int32_t n_ctas, void *stream) {
+    const ModeSpec ms = {"lstk_cuda_attn_decode_window", decode::kWindow, out_dtype, window, n_sink, nullptr, 0};
+    return decode_range(layout, k_cache, v_cache, q, q_dtype, n_seqs, n_head, block_tables, max_blocks_per_seq, seq_lens,
+                        max_seq_len, 0, INT32_MAX, scale, static_cast<float *>(out), lse_out, workspace,
+                        workspace_bytes, n_ctas, stream, nullptr, nullptr, &ms);
+}
+
+int lstk_cuda_attn_decode_window_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d,
+                                    const int8_t *v_qs, const void *v_d, const void *q, int32_t q_dtype,
+                                    int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                    int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len,
+                                    int32_t window, int32_t n_sink, float scale, void *out, int32_t out_dtype,
+                                    float *lse_out, void *workspace, size_t workspace_bytes, int32_t n_ctas,
+                                    void *stream) {
+    if (!k_qs || !k_d || !v_qs || !v_d)
+        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_decode_window_q8: NULL plane");
+    const Q8Planes q8 = {const_cast<int8_t *>(k_qs), const_cast<void *>(k_d), const_cast<int8_t *>(v_qs),
+                         const_cast<void *>(v_d)};
+    const ModeSpec ms = {"lstk_cuda_attn_decode_window_q8", decode::kWindow, out_dtype, window, n_sink, nullptr, 0};
+    return decode_range(layout, k_qs, v_qs, q, q_dtype, n_seqs, n_head, block_tables, max_blocks_per_seq, seq_lens,
+                        max_seq_len, 0, INT32_MAX, scale, static_cast<float *>(out), lse_out, workspace,
+                        workspace_bytes, n_ctas, stream, nullptr, &q8, &ms);
+}
+
+int lstk_cuda_attn_decode_weights(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
+                                  int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                  int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len, float scale,
+                                  float *acc, int64_t acc_stride, void *out, int32_t out_dtype, float *lse_out,
+                                  void *workspace, size_t workspace_bytes, int32_t n_ctas, void *stream) {
+    const ModeSpec ms = {"lstk_cuda_attn_decode_weights", decode::kWeights, out_dtype, 0, 0, acc, acc_stride};
+    return decode_range(layout, k_cache, v_cache, q, q_dtype, n_seqs, n_head, block_tables, max_blocks_per_seq, seq_lens,
+                        max_seq_len, 0, INT32_MAX, scale, static_cast<float *>(out), lse_out, workspace,
+                        workspace_bytes, n_ctas, stream, nullptr, nullptr, &ms);
+}
+
+int lstk_cuda_attn_decode_weights_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d,
+                                     const int8_t *v_qs, const void *v_d, const void *q, int32_t q_dtype,
+                                     int32_t n_seqs, int32_t n_head, const int32_t *block_tables,
+                                     int32_t max_blocks_per_seq, const int32_t *seq_lens, int32_t max_seq_len,
+                                     float scale, float *acc, int64_t acc_stride, void *out, int32_t out_dtype,
+                                     float *lse_out, void *workspace, size_t workspace_bytes, int32_t n_ctas,
+                                     void *stream) {
+    if (!k_qs || !k_d || !v_qs || !v_d)
+        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_decode_weights_q8: NULL plane");
+    const Q8Planes q8 = {const_cast<int8_t *>(k_qs), const_cast<void *>(k_d), const_cast<int8_t *>(v_qs),
+                         const_cast<void *>(v_d)};
+    const ModeSpec ms = {"lstk_cuda_attn_decode_weights_q8", decode::kWeights, out_dtype, 0, 0, acc, acc_stride};
+    return decode_range(layout, k_qs, v_qs, q, q_dtype, n_seqs, n_head, block_tables, max_blocks_per_seq, seq_lens,
+                        max_seq_len, 0, INT32_MAX, scale, static_cast<float *>(out), lse_out, workspace,
+                        workspace_bytes, n_ctas, stream, nullptr, &q8, &ms);
+}
 
 // Copies between ggml's block_q8_0 rows and the q8_0 planes (q8_layout.cuh).
 static int q8_convert(const void *src_a, const void *src_b, int64_t n_rows, void *dst_a, void *dst_b, bool to_blocks,

@@ -23,6 +23,20 @@ class Q8Cache:
         self.qs = torch.zeros((n_cells, n_head_kv, HEAD_DIM), dtype=torch.int8, device=device)
         self.d = torch.zeros((n_cells, n_head_kv, HEAD_DIM // 32), dtype=torch.float16, device=device)
 
+    @classmethod
+    def from_planes(cls, qs, d):
+        """A cache over existing planes (no copy): qs int8 [n_cells][n_head_kv][128], d f16
+        [n_cells][n_head_kv][4], both contiguous."""
+        if qs.dtype != torch.int8 or qs.dim() != 3 or qs.shape[2] != HEAD_DIM or qs.shape[0] % BLOCK_SIZE:
+            raise ValueError("qs must be int8 [n_cells][n_head_kv][128] with n_cells a multiple of 32")
+        if d.dtype != torch.float16 or d.shape != (*qs.shape[:2], HEAD_DIM // 32) or d.device != qs.device:
+            raise ValueError("d must be f16 [n_cells][n_head_kv][4] on the device of qs")
+        if not (qs.is_contiguous() and d.is_contiguous()):
+            raise ValueError("the planes must be contiguous")
+        c = cls.__new__(cls)
+        c.qs, c.d = qs, d
+        return c
+
     @property
     def layout(self):
         n_cells, hkv, hd = self.qs.shape

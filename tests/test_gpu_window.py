@@ -1,0 +1,140 @@
+"""Decode attention over a sliding window with sinks, against f64 (bounds: tests/bounded_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+import localstack_b200 as L
+from localstack_b200 import _lib
+from tests.bounded_ref import Batch, close, window_mask
+
+pytestmark = pytest.mark.gpu
+
+LENS = [0, 1, 31, 32, 33, 64, 100, 257, 1000]
+
+
+def _run(b, window, n_sink, **kw):
+    fn = L.attn_decode_window_q8 if b.q8 else L.attn_decode_window
+    out, lse = fn(*b.cache, b.q, b.bt, b.lens_t, window, n_sink, want_lse=True, **kw)
+    L.check_status()
+    return out, lse
+
+
+def _check(b, out, lse, window, n_sink):
+    bf16 = out.dtype == torch.bfloat16
+    out, lse = out.float().cpu().numpy(), lse.cpu().numpy()
+    for i in range(len(b.lens)):
+        o, l, _, t_o, t_l, _ = b.decode_ref(i, window, n_sink)
+        close(out[i:i + 1], o, t_o, bf16, f"out of length {b.lens[i]}")
+        close(lse[i:i + 1], l, t_l, False, f"lse of length {b.lens[i]}")
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("window,n_sink", [(1, 0), (1, 1), (16, 3), (31, 4), (32, 32), (33, 33), (100, 70), (256, 64),
+                                           (999, 1), (1000, 7), (5000, 4), (7, 5000), (2**31 - 1, 2**31 - 1)])
+def test_windows_and_sinks(window, n_sink, q8):
+    b = Batch(LENS, 32, 4, seed=window % 1000 + n_sink % 1000, q8=q8)
+    out, lse = _run(b, window, n_sink)
+    assert not out[0].any() and torch.isinf(lse[0]).all()  # no keys: zeros
+    _check(b, out, lse, window, n_sink)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(16, 8), (28, 4), (12, 2), (8, 1), (4, 4), (48, 12), (5, 5)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_dtype", [torch.float16, torch.float32])
+def test_heads_and_types(Hq, Hkv, out_dtype, q_dtype):
+    b = Batch([5, 700, 64, 333], Hq, Hkv, seed=Hq, q_dtype=q_dtype)
+    out, lse = _run(b, 130, 9, out_dtype=out_dtype)
+    assert out.dtype == out_dtype
+    _check(b, out, lse, 130, 9)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(16, 8), (28, 4), (12, 2), (20, 10)])
+def test_heads_q8_bf16(Hq, Hkv):
+    b = Batch([5, 700, 0, 333], Hq, Hkv, seed=Hq, q8=True)
+    out, lse = _run(b, 130, 9, out_dtype=torch.bfloat16)
+    _check(b, out, lse, 130, 9)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("lens", [[4000], [20000], [5000, 3, 17, 9000], list(range(1, 2000, 37))])
+@pytest.mark.parametrize("n_ctas", [0, 1, 7, 300])
+def test_splits(lens, n_ctas, q8):
+    """One long sequence over many CTAs (the combine's paths), a few, and a batch merged by rows."""
+    b = Batch(lens, 32, 4, seed=len(lens) + n_ctas, q8=q8)
+    out, lse = _run(b, 1500, 40, n_ctas=n_ctas, out_dtype=torch.bfloat16)
+    _check(b, out, lse, 1500, 40)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_hidden_cells_and_table_entries_do_not_matter(q8):
+    """NaN and infinities in every cell outside the window and the sinks (inside the visible pages
+    too), and page ids out of range in the gap: neither is looked at."""
+    lens, window, n_sink = [500, 77, 33, 1200, 64], 45, 5
+    b = Batch(lens, 16, 8, seed=3, q8=q8)
+    want, want_lse = _run(b, window, n_sink)
+    b.poison([np.flatnonzero(window_mask([n - 1], n, window, n_sink)[0]) for n in lens])
+    for i, n in enumerate(lens):
+        lo, hi = (n_sink + 31) // 32, max(0, n - window) // 32
+        b.bt[i, lo:max(lo, hi)] = -7
+        b.bt[i, (n + 31) // 32:] = 1 << 30
+    got, lse = _run(b, window, n_sink)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    _check(b, got, lse, window, n_sink)
+
+
+def test_a_window_over_everything_is_attn_decode():
+    """The same page-groups in the same split: the same bits as the whole-sequence decode."""
+    b = Batch(LENS + [3000], 32, 4, seed=5)
+    ref, ref_lse = L.attn_decode(*b.cache, b.q, b.bt, b.lens_t, want_lse=True)
+    for window, n_sink in ((3000, 0), (1, 3000), (2**31 - 1, 4)):
+        out, lse = _run(b, window, n_sink)
+        assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
+
+
+def test_bad_visible_page_and_length_are_reported():
+    b = Batch([300, 40], 32, 4, seed=6)
+    b.bt[0, 0] = 1 << 20  # the sinks' page
+    out = L.attn_decode_window(*b.cache, b.q, b.bt, b.lens_t, 50, 4)
+    with pytest.raises(L.LstkError) as e:
+        L.check_status()
+    assert e.value.code == _lib.LSTK_ERR_DEVICE_INDEX and torch.isfinite(out).all()
+    b = Batch([300, 40], 32, 4, seed=6)
+    b.lens_t[1] = 10 ** 6  # past the table: clamped to it
+    L.attn_decode_window(*b.cache, b.q, b.bt, b.lens_t, 50, 4)
+    with pytest.raises(L.LstkError):
+        L.check_status()
+
+
+def test_stream_graph_and_moving_lengths():
+    """Captured once with the lengths on the device, replayed as the sequences grow, on a side stream,
+    while another captured graph with a workspace of its own runs on the current one."""
+    window, n_sink = 64, 4
+    b = Batch([400, 90, 65], 32, 4, seed=8)
+    c = Batch([800], 16, 8, seed=9)
+    out, lse = torch.empty_like(b.q, dtype=torch.bfloat16), torch.empty(3, 32, device="cuda")
+    out_c = torch.empty_like(c.q, dtype=torch.float32)
+    ws, ws_c = L.DecodeWorkspace(3, 32, 4), L.DecodeWorkspace(1, 16, 8)
+    call = lambda: L.attn_decode_window(*b.cache, b.q, b.bt, b.lens_t, window, n_sink, out=out, lse_out=lse,  # noqa: E731
+                                        want_lse=True, workspace=ws)
+    call_c = lambda: L.attn_decode_window(*c.cache, c.q, c.bt, c.lens_t, 99, 1, out=out_c, workspace=ws_c)  # noqa: E731
+    call(), call_c()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graphs = []
+    for f in (call, call_c):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            f()
+        graphs.append(g)
+    for lens in ([400, 90, 65], [33, 64, 1], [0, 70, 66]):
+        b.lens = lens
+        b.lens_t.copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        L.check_status()
+        _check(b, out, lse, window, n_sink)
+        o, _, _, t, _, _ = c.decode_ref(0, 99, 1)
+        close(out_c.cpu().numpy(), o, t)
