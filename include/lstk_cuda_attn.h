@@ -361,6 +361,29 @@ int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, co
                            const int32_t *block_tables, int32_t max_blocks_per_seq, float scale, float *out,
                            void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- Prefill over a sliding window with sinks (no counterpart in the reference) --------------
+ * lstk_cuda_attn_prefill with the visibility of lstk_cuda_attn_decode_window: query token i, at
+ * position p, attends to keys j <= p, j < kv_lens[b], with j > p - window or j < n_sink (window >= 1,
+ * n_sink >= 0; a query that sees none gets zeros). Tiles between the sinks and the windows of a tile's
+ * queries are neither read nor computed, and block_tables entries of pages that no query sees are
+ * not looked at. out is f32 or bf16 (out_dtype; each f32 result rounded once). Cells that no query of
+ * a 128-row tile sees may hold anything; a non-finite K or V value that one of them does see may reach
+ * the tile's other rows. Other arguments, workspace and limits as lstk_cuda_attn_prefill; the _q8 form
+ * as lstk_cuda_attn_prefill_q8 (same scratch), dequantising only the pages that some query sees. */
+int lstk_cuda_attn_prefill_window(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache,
+                                  const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head,
+                                  const int32_t *q_seq_start, int32_t max_q_len, int64_t total_tokens,
+                                  const int32_t *q_pos0, const int32_t *kv_lens, const int32_t *block_tables,
+                                  int32_t max_blocks_per_seq, int32_t window, int32_t n_sink, float scale, void *out,
+                                  int32_t out_dtype, void *workspace, size_t workspace_bytes, void *stream);
+int lstk_cuda_attn_prefill_window_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d,
+                                     const int8_t *v_qs, const void *v_d, const void *q, int32_t q_dtype,
+                                     int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start, int32_t max_q_len,
+                                     int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
+                                     const int32_t *block_tables, int32_t max_blocks_per_seq, int32_t window,
+                                     int32_t n_sink, float scale, void *out, int32_t out_dtype, void *workspace,
+                                     size_t workspace_bytes, void *scratch, size_t scratch_bytes, void *stream);
+
 /* ---- Projections: replace attn_block's mul_mat nodes and the input RMSNorm ------------------
  * (src/qwen3.cpp:117-120 proj(), called at :135-138 for Wq / Wk / Wv and at :169 for Wo; the
  * residual add of :170; rms(x, attn_norm) of :112-114 / :134).

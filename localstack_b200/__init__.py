@@ -25,4 +25,6 @@ from .bounded import (  # noqa: F401,E402
     attn_decode_weights_q8,
     attn_decode_window,
     attn_decode_window_q8,
+    attn_prefill_window,
+    attn_prefill_window_q8,
 )

@@ -144,3 +144,67 @@ def attn_decode_weights_q8(kq: Q8Cache, vq: Q8Cache, q, block_tables, seq_lens, 
     layout, cache, device = _planes(kq, vq)
     return _decode_weights(lib().lstk_cuda_attn_decode_weights_q8, layout, cache, device, q, block_tables, seq_lens,
                            acc, scale, max_seq_len, out, out_dtype, lse_out, want_lse, workspace, n_ctas, stream)
+
+
+def _prefill_args(layout, q, q_seq_start, q_pos0, kv_lens, block_tables, max_q_len, out, out_dtype, workspace):
+    """Checks the shapes a prefill call relies on; returns (total, Hq, B, out, workspace), allocated when None."""
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype not in (torch.float16, torch.float32) or not q.is_contiguous():
+        raise ValueError("q must be a contiguous f16 or f32 tensor [total_tokens][Hq][128]")
+    total, Hq, _ = q.shape
+    B = q_pos0.numel()
+    for name, t in (("q_seq_start", q_seq_start), ("q_pos0", q_pos0), ("kv_lens", kv_lens),
+                    ("block_tables", block_tables)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor")
+    if q_seq_start.numel() != B + 1 or kv_lens.numel() != B or block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("q_seq_start [B+1], q_pos0 / kv_lens [B] and block_tables [B][max_blocks] must agree")
+    if out is None:
+        if out_dtype not in _OUT_DTYPES:
+            raise ValueError("out_dtype must be float32 or bfloat16")
+        out = torch.empty((total, Hq, HEAD_DIM), dtype=out_dtype, device=q.device)
+    elif out.dtype not in _OUT_DTYPES or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError("out must be a contiguous f32 or bf16 tensor of q's shape")
+    if q.dtype == torch.float32:  # the f16 copy of q lives in the workspace; f16 queries need none
+        need = lib().lstk_cuda_attn_prefill_workspace_size(B, Hq, layout.n_head_kv, HEAD_DIM, int(max_q_len),
+                                                           block_tables.shape[1], total, _DT[q.dtype])
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=q.device)
+    return total, Hq, B, out, workspace
+
+
+def attn_prefill_window(k_cache, v_cache, q, q_seq_start, q_pos0, kv_lens, block_tables, max_q_len, window, n_sink=0,
+                        scale=None, out=None, out_dtype=torch.float32, workspace=None, stream=None):
+    """attn_prefill restricted to a sliding window and sinks: the query at position p sees its last
+    `window` keys up to p (its own among them) and the first `n_sink`, all below kv_lens.
+
+    Tiles that no query sees are neither read nor computed. out (or out_dtype) is f32 or bf16; a query
+    that sees no key gets zeros. Other arguments as attn_prefill."""
+    layout, cache, device = _caches(k_cache, v_cache)
+    total, Hq, B, out, workspace = _prefill_args(layout, q, q_seq_start, q_pos0, kv_lens, block_tables, max_q_len, out,
+                                                 out_dtype, workspace)
+    check(lib().lstk_cuda_attn_prefill_window(
+        ctypes.byref(layout), *cache, _p(q), _DT[q.dtype], B, Hq, _p(q_seq_start), int(max_q_len), total, _p(q_pos0),
+        _p(kv_lens), _p(block_tables), block_tables.shape[1], int(window), int(n_sink),
+        _SCALE if scale is None else float(scale), _p(out), _DT[out.dtype], _p(workspace),
+        workspace.numel() if workspace is not None else 0, _stream(stream, device)))
+    return out
+
+
+def attn_prefill_window_q8(kq: Q8Cache, vq: Q8Cache, q, q_seq_start, q_pos0, kv_lens, block_tables, max_q_len, window,
+                           n_sink=0, scale=None, out=None, out_dtype=torch.float32, workspace=None, scratch=None,
+                           stream=None):
+    """attn_prefill_window over q8_0 planes: the pages that some query sees are dequantised into
+    `scratch` (uint8 of lstk_cuda_q8_prefill_scratch_size bytes, allocated when None) and the
+    tensor-core prefill runs on it, as attn_prefill_q8 does."""
+    layout, cache, device = _planes(kq, vq)
+    total, Hq, B, out, workspace = _prefill_args(layout, q, q_seq_start, q_pos0, kv_lens, block_tables, max_q_len, out,
+                                                 out_dtype, workspace)
+    need = lib().lstk_cuda_q8_prefill_scratch_size(B, block_tables.shape[1], layout.n_head_kv)
+    if scratch is None or scratch.numel() < need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    check(lib().lstk_cuda_attn_prefill_window_q8(
+        ctypes.byref(layout), *cache, _p(q), _DT[q.dtype], B, Hq, _p(q_seq_start), int(max_q_len), total, _p(q_pos0),
+        _p(kv_lens), _p(block_tables), block_tables.shape[1], int(window), int(n_sink),
+        _SCALE if scale is None else float(scale), _p(out), _DT[out.dtype], _p(workspace),
+        workspace.numel() if workspace is not None else 0, _p(scratch), scratch.numel(), _stream(stream, device)))
+    return out

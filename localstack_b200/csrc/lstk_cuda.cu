@@ -37,6 +37,7 @@ struct DeviceInfo {
     size_t decode_q8_smem = 0;
     size_t decode_mode_smem[2][3] = {};  // per [q8_0][mode] (windowed, with accumulated weights)
     size_t prefill_smem = 0;
+    size_t prefill_window_smem[2] = {};  // per out_dtype (f32, bf16)
     size_t append_smem[8] = {};  // per kv_append instantiation (append_kernel)
     size_t gemm_smem = 0;
     // Resident kv_append CTAs per SM, per [instantiation][rows per group / 4]; 0 = not asked yet.
@@ -891,30 +892,48 @@ size_t lstk_cuda_attn_prefill_workspace_size(int32_t n_seqs, int32_t n_head, int
     return align_up((size_t) total_tokens * n_head * head_dim * 2, 256);
 }
 
-int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
-                           int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start,
-                           int32_t max_q_len, int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
-                           const int32_t *block_tables, int32_t max_blocks_per_seq, float scale, float *out,
-                           void *workspace, size_t workspace_bytes, void *stream) {
-    int rc = check_layout(layout, "lstk_cuda_attn_prefill");
+// A prefill over a window with sinks (prefill.cuh's kWin).
+struct PrefillWindow {
+    const char *fn;
+    int32_t window, n_sink, out_dtype;
+};
+
+static int check_prefill_window(const PrefillWindow *pw, int32_t max_blocks_per_seq) {
+    if (pw->out_dtype != LSTK_DTYPE_F32 && pw->out_dtype != LSTK_DTYPE_BF16)
+        return set_error(LSTK_ERR_UNSUPPORTED, std::string(pw->fn) + ": out_dtype must be f32 or bf16");
+    if (pw->window < 1 || pw->n_sink < 0)
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(pw->fn) + ": window must be at least 1 and n_sink at least 0");
+    if (max_blocks_per_seq > INT32_MAX / 32)
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(pw->fn) + ": max_blocks_per_seq out of range");
+    return LSTK_OK;
+}
+
+static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
+                        int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start,
+                        int32_t max_q_len, int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
+                        const int32_t *block_tables, int32_t max_blocks_per_seq, float scale, float *out,
+                        void *workspace, size_t workspace_bytes, void *stream, const PrefillWindow *pw) {
+    const char *fn = pw ? pw->fn : "lstk_cuda_attn_prefill";
+    int rc = check_layout(layout, fn);
     if (rc) return rc;
+    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq))) return rc;
     const int hkv = layout->n_head_kv;
     if (n_seqs < 0 || n_head <= 0 || n_head % hkv != 0 || max_blocks_per_seq <= 0 || max_q_len < 0 ||
         total_tokens < 0 || total_tokens > (int64_t) INT32_MAX)
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_prefill: bad sizes");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad sizes");
     const int group = n_head / hkv;
     if (group > 8 || prefill::kBM % group != 0)
-        return set_error(LSTK_ERR_UNSUPPORTED, "lstk_cuda_attn_prefill: n_head / n_head_kv must be 1, 2, 4 or 8");
+        return set_error(LSTK_ERR_UNSUPPORTED, std::string(fn) + ": n_head / n_head_kv must be 1, 2, 4 or 8");
     if (q_dtype != LSTK_DTYPE_F16 && q_dtype != LSTK_DTYPE_F32)
-        return set_error(LSTK_ERR_UNSUPPORTED, "lstk_cuda_attn_prefill: q_dtype must be f16 or f32");
+        return set_error(LSTK_ERR_UNSUPPORTED, std::string(fn) + ": q_dtype must be f16 or f32");
     if (!k_cache || !v_cache || !q || !q_seq_start || !q_pos0 || !kv_lens || !block_tables || !out)
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_prefill: NULL pointer");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL pointer");
     if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(q, 16) || !aligned(out, 16))
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_prefill: misaligned pointer");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": misaligned pointer");
     if (workspace_bytes < lstk_cuda_attn_prefill_workspace_size(n_seqs, n_head, hkv, layout->head_dim, max_q_len,
                                                                 max_blocks_per_seq, total_tokens, q_dtype) ||
         (q_dtype == LSTK_DTYPE_F32 && (!workspace || !aligned(workspace, 256))))
-        return set_error(LSTK_ERR_CAPACITY, "lstk_cuda_attn_prefill: workspace too small or misaligned");
+        return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": workspace too small or misaligned");
     if (n_seqs == 0 || total_tokens == 0 || max_q_len == 0) return clear_error();
     DeviceInfo *dev = nullptr;
     if ((rc = bind_device(k_cache, &dev))) return rc;
@@ -933,7 +952,10 @@ int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, co
     CUtensorMap qmap, kmap, vmap, omap;
     const int tpt = prefill::kBM / group;
     if ((rc = encode_f16_3d(&qmap, q16, 128, n_head, total_tokens, 64, group, tpt))) return rc;
-    if ((rc = encode_f32_3d(&omap, out, 128, n_head, total_tokens, 32, group, tpt))) return rc;
+    const bool out16 = pw && pw->out_dtype == LSTK_DTYPE_BF16;
+    if ((rc = out16 ? encode_3d(&omap, out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 128, n_head, total_tokens, 64, group, tpt)
+                    : encode_f32_3d(&omap, out, 128, n_head, total_tokens, 32, group, tpt)))
+        return rc;
     if ((rc = encode_f16_3d(&kmap, k_cache, 128, hkv, layout->n_cells, 64, 1, 32))) return rc;
     if ((rc = encode_f16_3d(&vmap, v_cache, 128, hkv, layout->n_cells, 64, 1, 32))) return rc;
 
@@ -956,12 +978,17 @@ int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, co
     p.status = dev->status;
     p.wait_ns = t_pipeline_wait_ns;
     p.start_flag = t_start_flag;
+    p.window = pw ? pw->window : 0;
+    p.n_sink = pw ? pw->n_sink : 0;
     const int64_t n_items = (int64_t) n_seqs * p.n_qt * hkv;
-    if (n_items > (int64_t) INT32_MAX) return set_error(LSTK_ERR_CAPACITY, "lstk_cuda_attn_prefill: too many tiles");
+    if (n_items > (int64_t) INT32_MAX) return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": too many tiles");
     p.n_items = (int) n_items;
     // Persistent: one CTA per SM walks its share of the items (snake order over heaviest-first).
     const int64_t grid = std::min<int64_t>(n_items, dev->n_sms);
-    if ((rc = ensure_smem(&dev->prefill_smem, prefill::prefill_kernel, prefill::kSmemBytes,
+    const auto kernel = !pw     ? prefill::prefill_kernel<false, false>
+                        : out16 ? prefill::prefill_kernel<true, true>
+                                : prefill::prefill_kernel<true, false>;
+    if ((rc = ensure_smem(pw ? &dev->prefill_window_smem[out16] : &dev->prefill_smem, kernel, prefill::kSmemBytes,
                           "cudaFuncSetAttribute(prefill)")))
         return rc;
     cudaLaunchAttribute attr[1];
@@ -974,9 +1001,31 @@ int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, co
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return launch_pdl_check(cudaLaunchKernelEx(&cfg, prefill::prefill_kernel, qmap, kmap, vmap, omap, p),
-                            "prefill_kernel");
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, omap, p), "prefill_kernel");
 }
+
+int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
+                           int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start,
+                           int32_t max_q_len, int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
+                           const int32_t *block_tables, int32_t max_blocks_per_seq, float scale, float *out,
+                           void *workspace, size_t workspace_bytes, void *stream) {
+    return prefill_impl(layout, k_cache, v_cache, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len, total_tokens,
+                        q_pos0, kv_lens, block_tables, max_blocks_per_seq, scale, out, workspace, workspace_bytes,
+                        stream, nullptr);
+}
+
+int lstk_cuda_attn_prefill_window(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache,
+                                  const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head,
+                                  const int32_t *q_seq_start, int32_t max_q_len, int64_t total_tokens,
+                                  const int32_t *q_pos0, const int32_t *kv_lens, const int32_t *block_tables,
+                                  int32_t max_blocks_per_seq, int32_t window, int32_t n_sink, float scale, void *out,
+                                  int32_t out_dtype, void *workspace, size_t workspace_bytes, void *stream) {
+    const PrefillWindow pw = {"lstk_cuda_attn_prefill_window", window, n_sink, out_dtype};
+    return prefill_impl(layout, k_cache, v_cache, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len, total_tokens,
+                        q_pos0, kv_lens, block_tables, max_blocks_per_seq, scale, static_cast<float *>(out), workspace,
+                        workspace_bytes, stream, &pw);
+}
+
 
 // Scratch of lstk_cuda_attn_prefill_q8: the compact f16 K and V caches (n_seqs * max_blocks pages)
 // and their dense block tables, each 256-byte aligned.
@@ -990,23 +1039,27 @@ size_t lstk_cuda_q8_prefill_scratch_size(int32_t n_seqs, int32_t max_blocks_per_
            align_up(sizeof(int32_t) * (size_t) n_seqs * max_blocks_per_seq, 256);
 }
 
-int lstk_cuda_attn_prefill_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d, const int8_t *v_qs,
-                              const void *v_d, const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head,
-                              const int32_t *q_seq_start, int32_t max_q_len, int64_t total_tokens,
-                              const int32_t *q_pos0, const int32_t *kv_lens, const int32_t *block_tables,
-                              int32_t max_blocks_per_seq, float scale, float *out, void *workspace,
-                              size_t workspace_bytes, void *scratch, size_t scratch_bytes, void *stream) {
-    int rc = check_layout(layout, "lstk_cuda_attn_prefill_q8");
+static int prefill_q8_impl(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d, const int8_t *v_qs,
+                           const void *v_d, const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head,
+                           const int32_t *q_seq_start, int32_t max_q_len, int64_t total_tokens,
+                           const int32_t *q_pos0, const int32_t *kv_lens, const int32_t *block_tables,
+                           int32_t max_blocks_per_seq, float scale, float *out, void *workspace,
+                           size_t workspace_bytes, void *scratch, size_t scratch_bytes, void *stream,
+                           const PrefillWindow *pw) {
+    const char *fn = pw ? pw->fn : "lstk_cuda_attn_prefill_q8";
+    int rc = check_layout(layout, fn);
     if (rc) return rc;
+    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq))) return rc;
+    if (pw && (n_seqs > 0 && !q_pos0)) return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad arguments");
     if (!k_qs || !k_d || !v_qs || !v_d || !kv_lens || !block_tables || !scratch || n_seqs < 0 || max_blocks_per_seq <= 0)
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_prefill_q8: bad arguments");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad arguments");
     if (max_blocks_per_seq > 65535 || n_seqs > 65535)
-        return set_error(LSTK_ERR_CAPACITY, "lstk_cuda_attn_prefill_q8: more than 65535 sequences or pages per sequence");
+        return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": more than 65535 sequences or pages per sequence");
     if (!aligned(k_qs, 16) || !aligned(v_qs, 16) || !aligned(k_d, 2) || !aligned(v_d, 2) || !aligned(scratch, 256))
-        return set_error(LSTK_ERR_INVALID_ARG, "lstk_cuda_attn_prefill_q8: misaligned plane or scratch");
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": misaligned plane or scratch");
     const int hkv = layout->n_head_kv;
     if (scratch_bytes < lstk_cuda_q8_prefill_scratch_size(n_seqs, max_blocks_per_seq, hkv))
-        return set_error(LSTK_ERR_CAPACITY, "lstk_cuda_attn_prefill_q8: scratch too small");
+        return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": scratch too small");
     if (n_seqs == 0) return clear_error();
     DeviceInfo *dev = nullptr;
     if ((rc = bind_device(k_qs, &dev))) return rc;
@@ -1020,19 +1073,44 @@ int lstk_cuda_attn_prefill_q8(const lstk_kv_layout *layout, const int8_t *k_qs, 
     cfg.gridDim = dim3((unsigned) max_blocks_per_seq, (unsigned) n_seqs);
     cfg.blockDim = dim3(256);
     launch_pdl(cfg, attr, static_cast<cudaStream_t>(stream));
-    if ((rc = launch_pdl_check(cudaLaunchKernelEx(&cfg, q8::gather_dequant_kernel, k_qs,
+    if ((rc = launch_pdl_check(cudaLaunchKernelEx(&cfg, pw ? q8::gather_dequant_kernel<true> : q8::gather_dequant_kernel<false>, k_qs,
                                                   static_cast<const __half *>(k_d), v_qs,
                                                   static_cast<const __half *>(v_d), hkv,
                                                   (int64_t) (layout->n_cells / layout->block_size), block_tables,
-                                                  (int) max_blocks_per_seq, kv_lens, k16, v16, bt16, dev->status),
+                                                  (int) max_blocks_per_seq, kv_lens, k16, v16, bt16, dev->status, q_pos0,
+                                                  pw ? (int) pw->window : 0, pw ? (int) pw->n_sink : 0),
                                "q8 gather_dequant_kernel")))
         return rc;
     lstk_kv_layout l16 = *layout;
     l16.n_cells = (int64_t) n_seqs * max_blocks_per_seq * 32;
-    return lstk_cuda_attn_prefill(&l16, k16, v16, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len, total_tokens,
-                                  q_pos0, kv_lens, bt16, max_blocks_per_seq, scale, out, workspace, workspace_bytes,
-                                  stream);
+    return prefill_impl(&l16, k16, v16, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len, total_tokens, q_pos0,
+                        kv_lens, bt16, max_blocks_per_seq, scale, out, workspace, workspace_bytes, stream, pw);
 }
+
+int lstk_cuda_attn_prefill_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d, const int8_t *v_qs,
+                              const void *v_d, const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head,
+                              const int32_t *q_seq_start, int32_t max_q_len, int64_t total_tokens,
+                              const int32_t *q_pos0, const int32_t *kv_lens, const int32_t *block_tables,
+                              int32_t max_blocks_per_seq, float scale, float *out, void *workspace,
+                              size_t workspace_bytes, void *scratch, size_t scratch_bytes, void *stream) {
+    return prefill_q8_impl(layout, k_qs, k_d, v_qs, v_d, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len,
+                           total_tokens, q_pos0, kv_lens, block_tables, max_blocks_per_seq, scale, out, workspace,
+                           workspace_bytes, scratch, scratch_bytes, stream, nullptr);
+}
+
+int lstk_cuda_attn_prefill_window_q8(const lstk_kv_layout *layout, const int8_t *k_qs, const void *k_d,
+                                     const int8_t *v_qs, const void *v_d, const void *q, int32_t q_dtype,
+                                     int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start, int32_t max_q_len,
+                                     int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
+                                     const int32_t *block_tables, int32_t max_blocks_per_seq, int32_t window,
+                                     int32_t n_sink, float scale, void *out, int32_t out_dtype, void *workspace,
+                                     size_t workspace_bytes, void *scratch, size_t scratch_bytes, void *stream) {
+    const PrefillWindow pw = {"lstk_cuda_attn_prefill_window_q8", window, n_sink, out_dtype};
+    return prefill_q8_impl(layout, k_qs, k_d, v_qs, v_d, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len,
+                           total_tokens, q_pos0, kv_lens, block_tables, max_blocks_per_seq, scale,
+                           static_cast<float *>(out), workspace, workspace_bytes, scratch, scratch_bytes, stream, &pw);
+}
+
 
 static int pages_state(const lstk_kv_pages *st, pages::State *out) {
     if (!st || !st->free_blocks || !st->free_top || !st->block_tables || !st->seq_lens || !st->used_hwm ||

@@ -44,18 +44,23 @@ __global__ void __launch_bounds__(256) to_blocks_kernel(const uint16_t *qs, cons
 // Prefill over a q8_0 cache: the pages a call reads, dequantised into a compact f16 cache with
 // dense block tables (sequence b's page p -> scratch page b * max_blocks + p), which the f16
 // prefill then reads. CTA (p, b) converts one page of K and V (its keys below kv_lens[b]): 16
-// values per thread from one 16-byte load, each d * q rounded once to f16.
+// values per thread from one 16-byte load, each d * q rounded once to f16. kWin (window with sinks):
+// pages that no query of the sequence sees (its first query at q_pos0[b]) are left as they are; the
+// prefill does not read them.
+template <bool kWin>
 __global__ void __launch_bounds__(256) gather_dequant_kernel(const int8_t *k_qs, const __half *k_d, const int8_t *v_qs,
                                                              const __half *v_d, int hkv, int64_t n_pages_src,
                                                              const int32_t *block_tables, int max_blocks,
                                                              const int32_t *kv_lens, __half *k_out, __half *v_out,
-                                                             int32_t *bt_out, DeviceStatus *status) {
+                                                             int32_t *bt_out, DeviceStatus *status,
+                                                             const int32_t *q_pos0, int window, int n_sink) {
     pdl_wait();
     pdl_launch_dependents();
     const int p = blockIdx.x, b = blockIdx.y;
     const int64_t dst_page = (int64_t) b * max_blocks + p;
     if (threadIdx.x == 0) bt_out[dst_page] = (int32_t) dst_page;
     const int len = kv_lens[b];
+    if (kWin && p * 32 >= n_sink && (int64_t) p * 32 + 31 <= (int64_t) q_pos0[b] - window) return;
     const int32_t src_page = p * 32 < len ? block_tables[dst_page] : -1;
     const int64_t vals = (int64_t) 32 * hkv * 128;  // one page of one cache
     const int64_t dst0 = dst_page * vals;

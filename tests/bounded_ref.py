@@ -16,6 +16,13 @@ units, A = sum_i p_i |v_i| and V = sum_i |v_i| over the visible keys:
 pairwise and split partial sums stay far below 2^-17) and the log-sum-exp merges. The q8_0 decode
 computes exact integer dots scaled in f32, so E there is 16 * 2^-24 of the same magnitude, and
 rounds P * d_v to f16: the same relative bound, and 2^-25 * 127 absolute per key.
+
+The prefill multiplies on the tensor cores (a product sum may truncate: 2^-23 in E), rounds the scores
+less the running maximum (log2 units, at most 8 above zero, as far below as the key lies under the
+row's maximum) to f16 - ln 2 * 2^-11 * |x| of the probability - and takes ex2.approx.f16x2 of them
+(relative 2^-9.9); the row sum adds the same rounded probabilities, so with d_i the sum of these
+
+    |out - exact| <= sum_i p_i d_i (|v_i| + |out|) + 2^-25 sum_i (|v_i| + |out|)
 """
 from __future__ import annotations
 
@@ -59,32 +66,39 @@ def dequant(q, d):
     return q.astype(np.float64) * np.repeat(d.astype(np.float64), 32, axis=-1)
 
 
-def attend(q, k, v, seen, q8=False):
+def attend(q, k, v, seen, q8=False, prefill=False):
     """Exact attention of one sequence: q [T][Hq][128], k / v [S][Hkv][128] f64, seen [T][S]. Returns
     out, lse, weights [S] (summed over rows and heads) and the bounds of each (see above)."""
     T, Hq, D = q.shape
     G = Hq // k.shape[1]
-    out = np.zeros((T, Hq, D))
-    lse = np.full((T, Hq), -np.inf)
-    w = np.zeros(k.shape[0])
-    t_out, t_lse, t_w = np.zeros_like(out), np.zeros_like(lse), np.zeros_like(w)
-    for t in range(T):
-        i = np.flatnonzero(seen[t])
-        if not i.size:
-            continue
-        for h in range(Hq):
-            kk, vv = k[i, h // G], v[i, h // G]
-            x = kk @ q[t, h] * SCALE
-            m = x.max()
-            lse[t, h] = m + np.log(np.exp(x - m).sum())
-            p = np.exp(x - lse[t, h])
-            out[t, h] = p @ vv
-            E = SCALE * (16 if q8 else 128) * 2.0 ** -24 * (np.abs(kk) @ np.abs(q[t, h])).max()
-            t_out[t, h] = (2.0 ** -11 + 2 * E + 2.0 ** -16) * (p @ np.abs(vv)) + \
-                2.0 ** -25 * (127 * i.size if q8 else np.abs(vv).sum(0))
-            t_lse[t, h] = E + 2.0 ** -16 + 2.0 ** -22 * abs(lse[t, h])
-            w[i] += p
-            t_w[i] += (2 * E + 2.0 ** -16) * p
+    out, t_out = np.zeros((T, Hq, D)), np.zeros((T, Hq, D))
+    lse, t_lse = np.full((T, Hq), -np.inf), np.zeros((T, Hq))
+    w, t_w = np.zeros(k.shape[0]), np.zeros(k.shape[0])
+    rows, cols = np.flatnonzero(seen.any(1)), np.flatnonzero(seen.any(0))
+    if not rows.size:
+        return out, lse, w, t_out, t_lse, t_w
+    s = seen[np.ix_(rows, cols)]
+    for h in range(Hq):
+        kk, vv, qq = k[cols, h // G], v[cols, h // G], q[rows, h]
+        x = np.where(s, qq @ kk.T * SCALE, -np.inf)
+        m = x.max(1, keepdims=True)
+        e = np.exp(x - m)
+        l = m + np.log(e.sum(1, keepdims=True))
+        p = np.exp(x - l)
+        o = p @ vv
+        mag = np.where(s, np.abs(qq) @ np.abs(kk).T, 0.0).max(1, keepdims=True)
+        E = SCALE * (16 if q8 else 128) * 2.0 ** (-23 if prefill else -24) * mag
+        n, absv = s.sum(1, keepdims=True), np.abs(vv)
+        if prefill:
+            X = np.where(s, (m - x) / np.log(2.0), 0.0) + 8.0
+            d = np.log(2.0) * 2.0 ** -11 * X + 2.0 ** -9.9 + 2 * E + 2.0 ** -16
+            t = (p * d) @ absv + (p * d).sum(1, keepdims=True) * np.abs(o) + 2.0 ** -25 * (s @ absv + n * np.abs(o))
+        else:
+            t = (2.0 ** -11 + 2 * E + 2.0 ** -16) * (p @ absv) + 2.0 ** -25 * (127.0 * n if q8 else s @ absv)
+        out[rows, h], t_out[rows, h], lse[rows, h] = o, t, l[:, 0]
+        t_lse[rows, h] = (E + 2.0 ** -16 + 2.0 ** -22 * np.abs(l))[:, 0]
+        w[cols] += p.sum(0)
+        t_w[cols] += ((2 * E + 2.0 ** -16) * p).sum(0)
     return out, lse, w, t_out, t_lse, t_w
 
 

@@ -1,0 +1,146 @@
+"""Prefill attention over a sliding window with sinks, against f64 (bounds: tests/bounded_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+import localstack_b200 as L
+from localstack_b200 import _lib
+from tests.bounded_ref import Batch, attend, close, dequant, quantise_q8, vals, window_mask
+
+pytestmark = pytest.mark.gpu
+
+
+class Chunks:
+    """Sequences of (first query position, query tokens, keys)."""
+
+    def __init__(self, seqs, Hq, Hkv, seed=0, q8=False, q_dtype=torch.float16, spare_rows=0):
+        self.seqs = seqs
+        T = sum(t for _, t, _ in seqs)
+        self.b = Batch([n for _, _, n in seqs], Hq, Hkv, seed=seed, q8=q8, q_dtype=q_dtype, n_q=T + spare_rows)
+        b = self.b
+        if q8:  # the prefill of a q8_0 cache reads d * q rounded to f16, and f16 queries
+            planes = [quantise_q8(vals(x)) for x in (b.kb, b.vb)]
+            b.k_host, b.v_host = (dequant(*p).astype(np.float16).astype(np.float64) for p in planes)
+            b.q_host = b.q.half().cpu().numpy().astype(np.float64)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        self.starts = np.concatenate([[0], np.cumsum([t for _, t, _ in seqs])])
+        self.start_t, self.pos0_t = i32(self.starts.tolist()), i32([p for p, _, _ in seqs])
+        self.max_q = max(t for _, t, _ in seqs)
+
+    def run(self, window, n_sink, **kw):
+        b = self.b
+        fn = L.attn_prefill_window_q8 if b.q8 else L.attn_prefill_window
+        out = fn(*b.cache, b.q, self.start_t, self.pos0_t, b.lens_t, b.bt, self.max_q, window, n_sink, **kw)
+        L.check_status()
+        return out
+
+    def check(self, out, window, n_sink):
+        b, bf16 = self.b, out.dtype == torch.bfloat16
+        out = out.float().cpu().numpy()
+        for i, (p0, t, n) in enumerate(self.seqs):
+            rows = slice(self.starts[i], self.starts[i + 1])
+            c = b.cells(i)
+            seen = window_mask(p0 + np.arange(t), n, window, n_sink)
+            o, _, _, tol, _, _ = attend(b.q_host[rows], b.k_host[c], b.v_host[c], seen, prefill=True)
+            close(out[rows], o, tol, bf16, f"out of sequence {i}")
+
+
+RAGGED = [(0, 1, 1), (0, 70, 70), (31, 2, 33), (500, 129, 629), (0, 0, 5), (64, 64, 128), (1000, 17, 1017)]
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("window,n_sink", [(1, 0), (1, 1), (16, 5), (32, 32), (33, 4), (100, 70), (128, 0), (300, 64),
+                                           (5000, 4), (7, 5000), (2**31 - 1, 2**31 - 1)])
+def test_windows_and_sinks(window, n_sink, q8):
+    c = Chunks(RAGGED, 8, 2, seed=window % 1000 + n_sink % 1000, q8=q8)
+    c.check(c.run(window, n_sink), window, n_sink)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(8, 8), (8, 4), (32, 4), (16, 8), (8, 1)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("q_dtype", [torch.float16, torch.float32])
+def test_heads_and_types(Hq, Hkv, out_dtype, q_dtype):
+    c = Chunks([(300, 200, 500), (0, 77, 77)], Hq, Hkv, seed=Hq, q_dtype=q_dtype)
+    out = c.run(90, 5, out_dtype=out_dtype)
+    assert out.dtype == out_dtype
+    c.check(out, 90, 5)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_many_tiles_and_items(out_dtype):
+    """More items than SMs, windows of several tiles, sinks across pages."""
+    c = Chunks([(0, 1500, 1500), (2000, 700, 2700), (0, 333, 333)], 16, 8, seed=3)
+    c.check(c.run(640, 50, out_dtype=out_dtype), 640, 50)
+
+
+def test_rows_that_see_nothing_and_rows_of_no_sequence():
+    """Keys end before some queries' windows begin: those rows are zeros; spare rows are left alone."""
+    seqs = [(100, 100, 120), (500, 40, 100), (10, 30, 0)]
+    for out_dtype in (torch.float32, torch.bfloat16):
+        c = Chunks(seqs, 8, 2, seed=4, spare_rows=9)
+        out = torch.full((179, 8, 128), 7.0, dtype=out_dtype, device="cuda")
+        c.run(20, 0, out=out)
+        c.check(out[:170], 20, 0)
+        assert not out[40:170].any() and (out[170:] == 7).all()
+        assert out[:39].float().abs().sum((1, 2)).min() > 0
+        c.check(c.run(20, 3, out_dtype=out_dtype)[:170], 20, 3)
+
+
+def test_a_window_over_everything_is_attn_prefill():
+    c = Chunks(RAGGED, 8, 2, seed=5)
+    b = c.b
+    ref = L.attn_prefill(*b.cache, b.q, c.start_t, c.pos0_t, b.lens_t, b.bt, c.max_q)
+    assert torch.equal(c.run(1017, 0), ref) and torch.equal(c.run(2**31 - 1, 6), ref)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_hidden_cells_and_table_entries_do_not_matter(q8):
+    """NaN and infinities in every cell that no query of the sequence sees, one query tile each (G = 4:
+    32 tokens), and page ids out of range in the gap."""
+    seqs = [(500, 30, 530), (77, 1, 78), (10, 20, 30), (320, 32, 340)]
+    window, n_sink = 45, 5
+    c = Chunks(seqs, 8, 2, seed=6, q8=q8)
+    b = c.b
+    want = c.run(window, n_sink)
+    b.poison([np.flatnonzero(window_mask(p0 + np.arange(t), n, window, n_sink).any(0)) for p0, t, n in seqs])
+    for i, (p0, t, n) in enumerate(seqs):
+        lo, hi = (n_sink + 31) // 32, max(0, p0 + 1 - window) // 32
+        b.bt[i, lo:max(lo, hi)] = -7
+        b.bt[i, (n + 31) // 32:] = 1 << 30
+    got = c.run(window, n_sink)
+    assert torch.equal(got, want)
+    c.check(got, window, n_sink)
+
+
+def test_bad_page_and_rows_are_reported():
+    c = Chunks([(300, 64, 364), (0, 20, 20)], 8, 2, seed=7)
+    c.b.bt[0, 10] = 1 << 20
+    with pytest.raises(L.LstkError) as e:
+        c.run(60, 4)
+    assert e.value.code == _lib.LSTK_ERR_DEVICE_INDEX
+    c = Chunks([(300, 64, 364), (0, 20, 20)], 8, 2, seed=7)
+    c.start_t[2] = 1000  # rows behind the last one: the sequence is skipped
+    with pytest.raises(L.LstkError):
+        c.run(60, 4)
+
+
+def test_graph_on_another_stream():
+    c = Chunks([(0, 100, 100), (200, 30, 230)], 8, 2, seed=8, q_dtype=torch.float32)
+    b = c.b
+    out = torch.empty_like(b.q, dtype=torch.bfloat16)
+    ws = torch.empty(b.q.numel() * 2 + 256, dtype=torch.uint8, device="cuda")
+    c.run(40, 3, out=out, workspace=ws)
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=side):
+        L.attn_prefill_window(*b.cache, b.q, c.start_t, c.pos0_t, b.lens_t, b.bt, c.max_q, 40, 3, out=out, workspace=ws)
+    c.seqs = [(0, 100, 100), (150, 30, 180)]
+    c.pos0_t.copy_(torch.tensor([0, 150], dtype=torch.int32))
+    b.lens_t.copy_(torch.tensor([100, 180], dtype=torch.int32))
+    out.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        g.replay()
+    torch.cuda.synchronize()
+    L.check_status()
+    b.lens = [100, 180]
+    c.check(out, 40, 3)
