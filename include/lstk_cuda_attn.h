@@ -255,6 +255,56 @@ int lstk_cuda_kv_alloc(const lstk_kv_pages *state, const int32_t *slots, const i
                        int32_t max_tokens, int64_t *cells, int32_t *positions, int32_t *ok, void *stream);
 int lstk_cuda_kv_release(const lstk_kv_pages *state, int32_t slot, int32_t keep, void *stream);
 
+/* ---- Eviction by accumulated attention weight (no counterpart in the reference: its cache is full
+ * when its cells are used up, src/kv_cache.cpp:59-83) -------------------------------------------
+ * Holds every slot's sequence to `budget` keys by dropping the keys that the queries so far have
+ * attended to least. State per row (= slot of lstk_kv_pages), in caller-owned device memory, all zero
+ * for a new sequence:
+ *   acc    [n_rows][row_cells] f32: the weight that each cached key has received
+ *          (lstk_cuda_attn_decode_weights adds to it); entries at or past a row's length are zero
+ *   pos    [n_rows][row_cells] int32: the token position of the key at index i, for i < held
+ *   held   [n_rows] int32: indexes below it have their position in pos; the key at a later index i is
+ *          at position i + shift
+ *   shift  [n_rows] int32: tokens the row has lost so far: lstk_cuda_kv_alloc's position of a new token
+ *          plus shift is its position for lstk_cuda_kv_append
+ * A step of a serving loop whose rows have grown past the budget:
+ *   1. lstk_cuda_kv_evict_select: for every row with seq_lens[b] > budget, which keys stay - the tokens
+ *      at positions < n_sink, the last n_recent tokens, and then those of the largest acc (a NaN counts
+ *      as the smallest; equal ones by the lower index) up to `budget` keys - and the moves that bring
+ *      them below index budget: the j-th kept key at or past it (ascending) to the j-th index below it
+ *      whose key goes. n_moves [n_rows]; move_src / move_dst [n_rows][max_moves] indexes, -1 behind a
+ *      row's moves; max_moves >= min(budget, row_cells - budget). Changes nothing else. A row's keys
+ *      must not exceed row_cells (else it is reported, with no moves). n_sink + n_recent <= budget.
+ *   2. lstk_cuda_kv_move (or _q8) for each layer's cache: copies the moved rows of K and V through the
+ *      block tables. A move whose index or page is out of range is skipped and reported.
+ *   3. lstk_cuda_kv_evict_finish: moves acc and pos, clears acc behind the budget, advances held and
+ *      shift, and truncates the rows to budget (KvCache::truncate_seq in row order,
+ *      src/kv_cache.cpp:85-132: their blocks return to the free stack).
+ * The kept keys are then in no particular order, which decode attention does not see; a window
+ * (lstk_cuda_attn_decode_window) is taken over positions and does not apply to such a row. Set the
+ * row of a removed sequence back to zero (acc, held, shift) before its slot is used again. */
+typedef struct lstk_kv_weights {
+    float *acc;
+    int32_t *pos;
+    int32_t *held;
+    int32_t *shift;
+    int32_t n_rows;
+    int32_t row_cells;
+} lstk_kv_weights;
+int lstk_cuda_kv_evict_select(const lstk_kv_weights *weights, const int32_t *seq_lens, int32_t budget, int32_t n_sink,
+                              int32_t n_recent, int32_t max_moves, int32_t *n_moves, int32_t *move_src,
+                              int32_t *move_dst, void *stream);
+int lstk_cuda_kv_move(const lstk_kv_layout *layout, void *k_cache, void *v_cache, const int32_t *block_tables,
+                      int32_t n_rows, int32_t max_blocks_per_seq, const int32_t *n_moves, const int32_t *move_src,
+                      const int32_t *move_dst, int32_t max_moves, void *stream);
+int lstk_cuda_kv_move_q8(const lstk_kv_layout *layout, int8_t *k_qs, void *k_d, int8_t *v_qs, void *v_d,
+                         const int32_t *block_tables, int32_t n_rows, int32_t max_blocks_per_seq,
+                         const int32_t *n_moves, const int32_t *move_src, const int32_t *move_dst, int32_t max_moves,
+                         void *stream);
+int lstk_cuda_kv_evict_finish(const lstk_kv_pages *state, const lstk_kv_weights *weights, int32_t budget,
+                              const int32_t *n_moves, const int32_t *move_src, const int32_t *move_dst,
+                              int32_t max_moves, void *stream);
+
 /* ---- q8_0 KV cache (the reference's planned option, docs/plan.md:389-395; not built there) ----
  * The values of ggml's block_q8_0 (per 32 consecutive values of a row: d = amax / 127 kept as
  * f16, q = round-to-nearest-even(x / d) as int8 - quantize_row_q8_0's ARM form) in two planes per

@@ -28,3 +28,4 @@ from .bounded import (  # noqa: F401,E402
     attn_prefill_window,
     attn_prefill_window_q8,
 )
+from .evict import KvMoves, KvWeights, kv_move, kv_move_q8  # noqa: F401,E402

@@ -71,6 +71,12 @@ class KvPages(ctypes.Structure):
                 ("max_blocks", ctypes.c_int32), ("block_size", ctypes.c_int32)]
 
 
+class KvWeightsState(ctypes.Structure):
+    """lstk_kv_weights (include/lstk_cuda_attn.h): accumulated weights and positions of the cached keys."""
+    _fields_ = [("acc", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("held", ctypes.c_void_p),
+                ("shift", ctypes.c_void_p), ("n_rows", ctypes.c_int32), ("row_cells", ctypes.c_int32)]
+
+
 def declared_symbols():
     """Names of every function declared in include/lstk_cuda_attn.h."""
     with open(HEADER) as f:
@@ -144,6 +150,10 @@ def lib():
     L.lstk_cuda_rms_norm.argtypes = [_P, _I32, _I64, _P, _F, _P, _I64, _I32, _I32, _P]
     L.lstk_cuda_to_bf16.argtypes = [_P, _I64, _P, _I64, _I32, _I32, _P]
     L.lstk_cuda_kv_alloc.argtypes = [_P, _P, _P, _I32, _I32, _P, _P, _P, _P]
+    L.lstk_cuda_kv_evict_select.argtypes = [_P, _P, _I32, _I32, _I32, _I32, _P, _P, _P, _P]
+    L.lstk_cuda_kv_move.argtypes = [_LP, _P, _P, _P, _I32, _I32, _P, _P, _P, _I32, _P]
+    L.lstk_cuda_kv_move_q8.argtypes = [_LP, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P, _I32, _P]
+    L.lstk_cuda_kv_evict_finish.argtypes = [_P, _P, _I32, _P, _P, _P, _I32, _P]
     L.lstk_cuda_kv_release.argtypes = [_P, _I32, _I32, _P]
     _lib = L
     return L

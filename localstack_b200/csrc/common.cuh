@@ -44,6 +44,9 @@ enum : int {
     kSiteGemmSmem = 51,
     kSitePagesSlot = 40,
     kSitePagesTokens = 41,
+    kSiteEvictLen = 60,
+    kSiteEvictMove = 61,
+    kSiteEvictPage = 62,
 };
 
 __device__ __forceinline__ void report(DeviceStatus *st, int code, int where, int detail) {

@@ -3,6 +3,7 @@
 // (except lstk_cuda_status, whose job is to synchronise and read the device status word).
 #include "common.cuh"
 #include "decode.cuh"
+#include "evict.cuh"
 #include "exchange.cuh"
 #include "gemm.cuh"
 #include "host_util.h"
@@ -40,6 +41,7 @@ struct DeviceInfo {
     size_t prefill_window_smem[2] = {};  // per out_dtype (f32, bf16)
     size_t append_smem[8] = {};  // per kv_append instantiation (append_kernel)
     size_t gemm_smem = 0;
+    size_t evict_smem = 0;
     // Resident kv_append CTAs per SM, per [instantiation][rows per group / 4]; 0 = not asked yet.
     int append_occ[8][append::kMaxGroupRows / 4 + 1] = {};
 };
@@ -908,15 +910,12 @@ static int check_prefill_window(const PrefillWindow *pw, int32_t max_blocks_per_
     return LSTK_OK;
 }
 
-static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
-                        int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start,
-                        int32_t max_q_len, int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
-                        const int32_t *block_tables, int32_t max_blocks_per_seq, float scale, float *out,
-                        void *workspace, size_t workspace_bytes, void *stream, const PrefillWindow *pw) {
-    const char *fn = pw ? pw->fn : "lstk_cuda_attn_prefill";
-    int rc = check_layout(layout, fn);
-    if (rc) return rc;
-    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq))) return rc;
+// What the prefill entry points ask of their arguments (layout checked before).
+static int check_prefill(const char *fn, const lstk_kv_layout *layout, const void *k_cache, const void *v_cache,
+                         const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start,
+                         int32_t max_q_len, int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
+                         const int32_t *block_tables, int32_t max_blocks_per_seq, const float *out,
+                         const void *workspace, size_t workspace_bytes) {
     const int hkv = layout->n_head_kv;
     if (n_seqs < 0 || n_head <= 0 || n_head % hkv != 0 || max_blocks_per_seq <= 0 || max_q_len < 0 ||
         total_tokens < 0 || total_tokens > (int64_t) INT32_MAX)
@@ -934,6 +933,23 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
                                                                 max_blocks_per_seq, total_tokens, q_dtype) ||
         (q_dtype == LSTK_DTYPE_F32 && (!workspace || !aligned(workspace, 256))))
         return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": workspace too small or misaligned");
+    return LSTK_OK;
+}
+
+static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
+                        int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start,
+                        int32_t max_q_len, int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
+                        const int32_t *block_tables, int32_t max_blocks_per_seq, float scale, float *out,
+                        void *workspace, size_t workspace_bytes, void *stream, const PrefillWindow *pw) {
+    const char *fn = pw ? pw->fn : "lstk_cuda_attn_prefill";
+    int rc = check_layout(layout, fn);
+    if (rc) return rc;
+    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq))) return rc;
+    if ((rc = check_prefill(fn, layout, k_cache, v_cache, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len,
+                            total_tokens, q_pos0, kv_lens, block_tables, max_blocks_per_seq, out, workspace,
+                            workspace_bytes)))
+        return rc;
+    const int hkv = layout->n_head_kv, group = n_head / hkv;
     if (n_seqs == 0 || total_tokens == 0 || max_q_len == 0) return clear_error();
     DeviceInfo *dev = nullptr;
     if ((rc = bind_device(k_cache, &dev))) return rc;
@@ -1050,7 +1066,10 @@ static int prefill_q8_impl(const lstk_kv_layout *layout, const int8_t *k_qs, con
     int rc = check_layout(layout, fn);
     if (rc) return rc;
     if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq))) return rc;
-    if (pw && (n_seqs > 0 && !q_pos0)) return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad arguments");
+    if (pw && (rc = check_prefill(fn, layout, k_qs, v_qs, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len,
+                                  total_tokens, q_pos0, kv_lens, block_tables, max_blocks_per_seq, out, workspace,
+                                  workspace_bytes)))
+        return rc;
     if (!k_qs || !k_d || !v_qs || !v_d || !kv_lens || !block_tables || !scratch || n_seqs < 0 || max_blocks_per_seq <= 0)
         return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad arguments");
     if (max_blocks_per_seq > 65535 || n_seqs > 65535)
@@ -1147,6 +1166,172 @@ int lstk_cuda_kv_release(const lstk_kv_pages *state, int32_t slot, int32_t keep,
     if ((rc = bind_device(state->block_tables, &dev))) return rc;
     pages::release_kernel<<<1, pages::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(st, slot, keep);
     return launch_check("release_kernel");
+}
+
+// ---- eviction by accumulated weight (evict.cuh) ------------------------------------------------
+
+static int evict_weights(const lstk_kv_weights *w, const char *fn, evict::Weights *out) {
+    if (!w || !w->acc || !w->pos || !w->held || !w->shift || w->n_rows < 0 || w->row_cells <= 0)
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad weights");
+    *out = {w->acc, w->pos, w->held, w->shift, w->n_rows, w->row_cells};
+    return LSTK_OK;
+}
+
+// Moves a row can have: a mover lies at or past the budget, a hole below it.
+static int32_t evict_most_moves(int32_t budget, int32_t row_cells) {
+    return std::max(0, std::min(budget, row_cells - budget));
+}
+
+int lstk_cuda_kv_evict_select(const lstk_kv_weights *weights, const int32_t *seq_lens, int32_t budget, int32_t n_sink,
+                              int32_t n_recent, int32_t max_moves, int32_t *n_moves, int32_t *move_src,
+                              int32_t *move_dst, void *stream) {
+    const char *fn = "lstk_cuda_kv_evict_select";
+    evict::SelectParams p;
+    int rc = evict_weights(weights, fn, &p.w);
+    if (rc) return rc;
+    if (budget < 1 || n_sink < 0 || n_recent < 0 || (int64_t) n_sink + n_recent > budget)
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": the budget must be at least 1 and hold n_sink + n_recent keys");
+    if (max_moves < evict_most_moves(budget, weights->row_cells))
+        return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": max_moves below min(budget, row_cells - budget)");
+    if (!seq_lens || !n_moves || (max_moves > 0 && (!move_src || !move_dst)))
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL pointer");
+    if (weights->n_rows == 0) return clear_error();
+    DeviceInfo *dev = nullptr;
+    if ((rc = bind_device(weights->acc, &dev))) return rc;
+    p.seq_lens = seq_lens;
+    p.budget = budget;
+    p.n_sink = n_sink;
+    p.n_recent = n_recent;
+    p.max_moves = max_moves;
+    p.n_moves = n_moves;
+    p.src = move_src;
+    p.dst = move_dst;
+    p.status = dev->status;
+    // CTAs per row: one per 4096 cells, up to the portable cluster size of 8
+    int cluster = 1;
+    while (cluster < 8 && (int64_t) cluster * 4096 < weights->row_cells) cluster *= 2;
+    p.cap = std::min((weights->row_cells + cluster - 1) / cluster, 32768);
+    const size_t smem = sizeof(uint32_t) * (size_t) p.cap;
+    if ((int64_t) weights->n_rows * cluster > (int64_t) INT32_MAX)
+        return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": too many rows");
+    if ((rc = ensure_smem(&dev->evict_smem, evict::select_kernel, smem, "cudaFuncSetAttribute(evict)"))) return rc;
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) (weights->n_rows * cluster));
+    cfg.blockDim = dim3(evict::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    launch_pdl(cfg, attr, static_cast<cudaStream_t>(stream));
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned) cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg, evict::select_kernel, p), "evict select_kernel");
+}
+
+static int kv_move_impl(const char *fn, const lstk_kv_layout *layout, evict::MoveParams &p, const int32_t *block_tables,
+                        int32_t n_rows, int32_t max_blocks_per_seq, const int32_t *n_moves, const int32_t *move_src,
+                        const int32_t *move_dst, int32_t max_moves, void *stream) {
+    if (n_rows < 0 || max_blocks_per_seq <= 0 || max_blocks_per_seq > INT32_MAX / 32 || max_moves < 0)
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad sizes");
+    if (!block_tables || !n_moves || (max_moves > 0 && (!move_src || !move_dst)))
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL pointer");
+    if (n_rows == 0 || max_moves == 0) return clear_error();
+    DeviceInfo *dev = nullptr;
+    int rc = bind_device(p.plane[0], &dev);
+    if (rc) return rc;
+    p.block_tables = block_tables;
+    p.n_rows = n_rows;
+    p.max_blocks = max_blocks_per_seq;
+    p.n_pages = layout->n_cells / layout->block_size;
+    p.n_moves = n_moves;
+    p.src = move_src;
+    p.dst = move_dst;
+    p.max_moves = max_moves;
+    p.status = dev->status;
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = {};
+    const int64_t warps = (int64_t) n_rows * max_moves;
+    cfg.gridDim = dim3((unsigned) std::min<int64_t>((warps + evict::kMoveThreads / 32 - 1) / (evict::kMoveThreads / 32),
+                                                    (int64_t) dev->n_sms * 16));
+    cfg.blockDim = dim3(evict::kMoveThreads);
+    launch_pdl(cfg, attr, static_cast<cudaStream_t>(stream));
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg, evict::move_kernel, p), "evict move_kernel");
+}
+
+int lstk_cuda_kv_move(const lstk_kv_layout *layout, void *k_cache, void *v_cache, const int32_t *block_tables,
+                      int32_t n_rows, int32_t max_blocks_per_seq, const int32_t *n_moves, const int32_t *move_src,
+                      const int32_t *move_dst, int32_t max_moves, void *stream) {
+    const char *fn = "lstk_cuda_kv_move";
+    int rc = check_layout(layout, fn);
+    if (rc) return rc;
+    if (!k_cache || !v_cache) return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL pointer");
+    if (!aligned(k_cache, 16) || !aligned(v_cache, 16))
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": misaligned pointer");
+    evict::MoveParams p = {};
+    const int row = layout->n_head_kv * layout->head_dim * 2;
+    p.plane[0] = static_cast<uint8_t *>(k_cache);
+    p.plane[1] = static_cast<uint8_t *>(v_cache);
+    p.row_bytes[0] = p.row_bytes[1] = row;
+    p.n_planes = 2;
+    return kv_move_impl(fn, layout, p, block_tables, n_rows, max_blocks_per_seq, n_moves, move_src, move_dst, max_moves,
+                        stream);
+}
+
+int lstk_cuda_kv_move_q8(const lstk_kv_layout *layout, int8_t *k_qs, void *k_d, int8_t *v_qs, void *v_d,
+                         const int32_t *block_tables, int32_t n_rows, int32_t max_blocks_per_seq,
+                         const int32_t *n_moves, const int32_t *move_src, const int32_t *move_dst, int32_t max_moves,
+                         void *stream) {
+    const char *fn = "lstk_cuda_kv_move_q8";
+    int rc = check_layout(layout, fn);
+    if (rc) return rc;
+    if (!k_qs || !k_d || !v_qs || !v_d) return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL plane");
+    if (!aligned(k_qs, 16) || !aligned(v_qs, 16) || !aligned(k_d, 8) || !aligned(v_d, 8))
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": misaligned plane");
+    evict::MoveParams p = {};
+    p.plane[0] = reinterpret_cast<uint8_t *>(k_qs);
+    p.plane[1] = reinterpret_cast<uint8_t *>(v_qs);
+    p.plane[2] = static_cast<uint8_t *>(k_d);
+    p.plane[3] = static_cast<uint8_t *>(v_d);
+    p.row_bytes[0] = p.row_bytes[1] = layout->n_head_kv * layout->head_dim;
+    p.row_bytes[2] = p.row_bytes[3] = layout->n_head_kv * (layout->head_dim / 32) * 2;
+    p.n_planes = 4;
+    return kv_move_impl(fn, layout, p, block_tables, n_rows, max_blocks_per_seq, n_moves, move_src, move_dst, max_moves,
+                        stream);
+}
+
+int lstk_cuda_kv_evict_finish(const lstk_kv_pages *state, const lstk_kv_weights *weights, int32_t budget,
+                              const int32_t *n_moves, const int32_t *move_src, const int32_t *move_dst,
+                              int32_t max_moves, void *stream) {
+    const char *fn = "lstk_cuda_kv_evict_finish";
+    evict::FinishParams p;
+    pages::State st;
+    int rc = evict_weights(weights, fn, &p.w);
+    if (rc || (rc = pages_state(state, &st))) return rc;
+    if (budget < 1 || max_moves < evict_most_moves(budget, weights->row_cells))
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": bad budget / max_moves");
+    if (state->n_slots != weights->n_rows || state->max_blocks > INT32_MAX / pages::kBlock ||
+        state->max_blocks * pages::kBlock > weights->row_cells)
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": the weights' rows must be the slots, and hold their cells");
+    if (!n_moves || (max_moves > 0 && (!move_src || !move_dst)))
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL pointer");
+    DeviceInfo *dev = nullptr;
+    if ((rc = bind_device(state->block_tables, &dev))) return rc;
+    p.seq_lens = st.seq_lens;
+    p.max_len = state->max_blocks * pages::kBlock;
+    p.budget = budget;
+    p.n_moves = n_moves;
+    p.src = move_src;
+    p.dst = move_dst;
+    p.max_moves = max_moves;
+    p.status = dev->status;
+    cudaLaunchAttribute attr[1];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) weights->n_rows);
+    cfg.blockDim = dim3(evict::kThreads);
+    launch_pdl(cfg, attr, static_cast<cudaStream_t>(stream));
+    if ((rc = launch_pdl_check(cudaLaunchKernelEx(&cfg, evict::finish_kernel, p), "evict finish_kernel"))) return rc;
+    cfg.gridDim = dim3(1);
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg, evict::truncate_kernel, st, (int) budget), "evict truncate_kernel");
 }
 
 size_t lstk_cuda_mailbox_bytes(int32_t n_ranks, int64_t n_rows, int32_t head_dim) {

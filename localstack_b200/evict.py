@@ -1,0 +1,137 @@
+"""Eviction from the paged cache by accumulated attention weight (lstk_kv_weights,
+include/lstk_cuda_attn.h).
+
+A serving loop adds up what each cached key receives (bounded.attn_decode_weights on KvWeights.acc),
+and when rows have grown past their budget drops the keys with the smallest sums:
+
+    moves = weights.select(pages.seq_lens, budget, n_sink, n_recent)   # which keys stay
+    for k, v in layers: kv_move(k, v, pages.block_tables, moves)        # their K and V rows
+    weights.finish(pages, moves)                                        # lengths, blocks, acc, positions
+
+The reference has no counterpart: its cache is full when its cells are used up
+(src/kv_cache.cpp:59-83).
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import KvWeightsState, check, lib
+from .attn import _p, _stream
+from .bounded import _caches, _planes
+from .q8 import Q8Cache
+
+BLOCK = 32
+
+
+@dataclass
+class KvMoves:
+    """The moves of one eviction: row b's key at index src[b][j] goes to index dst[b][j], j < n[b]; entries
+    behind them are -1. int32 device tensors [rows], [rows][max_moves], [rows][max_moves]."""
+
+    n: torch.Tensor
+    src: torch.Tensor
+    dst: torch.Tensor
+    budget: int
+
+
+class KvWeights:
+    """Accumulated weights and token positions of the cached keys of n_rows slots (one row per slot of a
+    DevicePages of max_blocks blocks a slot), zero for new sequences.
+
+    acc f32 [n_rows][cells]: pass it to attn_decode_weights. pos int32 [n_rows][cells], held and shift
+    int32 [n_rows]: the key at index i is the token at position pos[i] (i < held) or i + shift."""
+
+    def __init__(self, n_rows, max_blocks, device="cuda"):
+        cells = max_blocks * BLOCK
+        self._set(torch.zeros((n_rows, cells), dtype=torch.float32, device=device),
+                  torch.zeros((n_rows, cells), dtype=torch.int32, device=device),
+                  torch.zeros(n_rows, dtype=torch.int32, device=device),
+                  torch.zeros(n_rows, dtype=torch.int32, device=device))
+
+    @classmethod
+    def from_tensors(cls, acc, pos, held, shift):
+        """A state over existing tensors (no copy)."""
+        if acc.dtype != torch.float32 or acc.dim() != 2:
+            raise ValueError("acc must be f32 [rows][cells]")
+        if any(t.dtype != torch.int32 for t in (pos, held, shift)):
+            raise ValueError("pos, held and shift must be int32")
+        if pos.shape != acc.shape or held.shape != acc.shape[:1] or shift.shape != acc.shape[:1]:
+            raise ValueError("pos must be [rows][cells], held and shift [rows]")
+        if any(not t.is_contiguous() or t.device != acc.device for t in (acc, pos, held, shift)):
+            raise ValueError("acc, pos, held and shift must be contiguous, on one device")
+        w = cls.__new__(cls)
+        w._set(acc, pos, held, shift)
+        return w
+
+    def _set(self, acc, pos, held, shift):
+        self.acc, self.pos, self.held, self.shift = acc, pos, held, shift
+        self.n_rows, self.row_cells = acc.shape
+        self.device = acc.device
+        self.state = KvWeightsState(acc.data_ptr(), pos.data_ptr(), held.data_ptr(), shift.data_ptr(), self.n_rows,
+                                    self.row_cells)
+
+    def select(self, seq_lens, budget, n_sink=0, n_recent=0, moves=None, stream=None):
+        """The moves that hold every row to `budget` keys: tokens at positions < n_sink and the last
+        n_recent stay, then the largest acc (lower index first among equal ones). Rows at or below the
+        budget have none. `moves` (an earlier result for the same sizes) is written again if given."""
+        budget = int(budget)
+        if seq_lens.dtype != torch.int32 or seq_lens.numel() != self.n_rows or not seq_lens.is_contiguous():
+            raise ValueError("seq_lens must be a contiguous int32 tensor, one per row")
+        most = max(0, min(budget, self.row_cells - budget))
+        if moves is None:
+            room = torch.empty(self.n_rows * (2 * most + 1), dtype=torch.int32, device=self.device)
+            n, src, dst = room.split((self.n_rows, self.n_rows * most, self.n_rows * most))
+            moves = KvMoves(n, src.view(self.n_rows, most), dst.view(self.n_rows, most), budget)
+        elif (moves.src.shape != moves.dst.shape or moves.src.shape[0] != self.n_rows or moves.src.shape[1] < most
+              or moves.n.numel() != self.n_rows
+              or any(t.dtype != torch.int32 or not t.is_contiguous() for t in (moves.n, moves.src, moves.dst))):
+            raise ValueError("moves must hold min(budget, cells - budget) moves for every row")
+        check(lib().lstk_cuda_kv_evict_select(ctypes.byref(self.state), _p(seq_lens), budget, int(n_sink),
+                                              int(n_recent), moves.src.shape[1], _p(moves.n), _p(moves.src),
+                                              _p(moves.dst), _stream(stream, self.device)))
+        moves.budget = budget
+        return moves
+
+    def finish(self, pages, moves, stream=None):
+        """Ends an eviction: acc and pos follow the moves, the rows of `pages` (a DevicePages) are
+        truncated to the budget and their blocks freed. Call it once, after every layer's kv_move."""
+        if moves.src.shape[0] != self.n_rows:
+            raise ValueError("moves and weights must have the same rows")
+        check(lib().lstk_cuda_kv_evict_finish(ctypes.byref(pages.state), ctypes.byref(self.state), moves.budget,
+                                              _p(moves.n), _p(moves.src), _p(moves.dst), moves.src.shape[1],
+                                              _stream(stream, self.device)))
+
+    def positions(self, positions, slots):
+        """Token positions (for kv_append's RoPE) of new tokens that DevicePages.alloc placed at
+        `positions`, one slot index per token."""
+        return positions + self.shift[slots.long()]
+
+    def reset(self, slot):
+        """Clears the row of a removed sequence, on the current stream."""
+        self.acc[slot].zero_()
+        self.held[slot].zero_()
+        self.shift[slot].zero_()
+
+
+def _move(fn, layout, cache, device, block_tables, moves, stream):
+    rows = moves.src.shape[0]
+    if block_tables.dtype != torch.int32 or not block_tables.is_contiguous() or block_tables.dim() != 2 \
+            or block_tables.shape[0] != rows:
+        raise ValueError("block_tables must be a contiguous int32 [rows][max_blocks] tensor")
+    check(fn(ctypes.byref(layout), *cache, _p(block_tables), rows, block_tables.shape[1], _p(moves.n), _p(moves.src),
+             _p(moves.dst), moves.src.shape[1], _stream(stream, device)))
+
+
+def kv_move(k_cache, v_cache, block_tables, moves: KvMoves, stream=None):
+    """Carries out an eviction's moves on one layer's K and V caches (f16 [n_cells][n_head_kv][128])."""
+    layout, cache, device = _caches(k_cache, v_cache)
+    _move(lib().lstk_cuda_kv_move, layout, cache, device, block_tables, moves, stream)
+
+
+def kv_move_q8(kq: Q8Cache, vq: Q8Cache, block_tables, moves: KvMoves, stream=None):
+    """kv_move on q8_0 planes."""
+    layout, cache, device = _planes(kq, vq)
+    _move(lib().lstk_cuda_kv_move_q8, layout, cache, device, block_tables, moves, stream)
