@@ -1440,17 +1440,23 @@ __global__ void __launch_bounds__(kAccumulateThreads) weights_accumulate_kernel(
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int n_pages = p.prefix[p.n_seqs];
-    for (int y = blockIdx.x * (kAccumulateThreads / 32) + (threadIdx.x >> 5); y < n_pages;
-         y += gridDim.x * (kAccumulateThreads / 32)) {
-        int lo = 0, hi = p.n_seqs;  // largest b with prefix[b] <= y: the sequence that holds page y
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (p.prefix[mid] <= y) lo = mid; else hi = mid - 1;
-        }
-        const int b = lo, pb = p.prefix[b], np = p.prefix[b + 1] - pb, pg = y - pb;
+    // this warp's stretch of pages
+    const int64_t W = (int64_t) gridDim.x * (kAccumulateThreads / 32);
+    const int64_t me = (int64_t) blockIdx.x * (kAccumulateThreads / 32) + (threadIdx.x >> 5);
+    const int y0 = (int) (me * n_pages / W), y1 = (int) ((me + 1) * n_pages / W);
+    if (y0 == y1) return;
+    int b = 0;
+    for (int hi = p.n_seqs; b < hi;) {  // largest b with prefix[b] <= y0: the sequence that holds page y0
+        const int mid = (b + hi + 1) >> 1;
+        if (p.prefix[mid] <= y0) b = mid; else hi = mid - 1;
+    }
+    for (int y = y0; y < y1; y++) {
+        while (p.prefix[b + 1] <= y) b++;
+        const int pb = p.prefix[b], np = p.prefix[b + 1] - pb, pg = y - pb;
         const int len = min(max(p.seq_lens[b], 0), p.max_len);
         const bool live = pg * kPage + lane < len;
-        float w = 0.f;
+        float *acc = p.acc + (int64_t) b * p.acc_stride + pg * kPage + lane;
+        float w = live ? *acc : 0.f, add = 0.f;
         for (int hg = 0; hg < p.n_hg; hg++) {
             const int rows = min(kHeadsPerGroup, p.n_head_kv - hg * kHeadsPerGroup) * p.group;
             const int64_t x = (int64_t) p.n_hg * pb + (int64_t) hg * np + pg;
@@ -1459,13 +1465,18 @@ __global__ void __launch_bounds__(kAccumulateThreads) weights_accumulate_kernel(
             const float l = lane < rows ? p.lse[(int64_t) b * p.n_head + (int64_t) hg * kHeadsPerGroup * p.group + lane]
                                         : -INFINITY;
             const float l2 = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
-#pragma unroll 8
-            for (int r = 0; r < rows; r++) {
-                const float lr = __shfl_sync(0xffffffffu, l2, r);
-                if (live) w += fast_exp2(rec[r * kPage] - lr);
+            for (int r0 = 0; r0 < rows; r0 += 16) {
+                float s[16];
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = live && r0 + r < rows ? rec[(r0 + r) * kPage] : -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float lr = __shfl_sync(0xffffffffu, l2, (r0 + r) & 31);
+                    if (r0 + r < rows) add += fast_exp2(s[r] - lr);
+                }
             }
         }
-        if (live) p.acc[(int64_t) b * p.acc_stride + pg * kPage + lane] += w;
+        if (live) *acc = w + add;
     }
 }
 

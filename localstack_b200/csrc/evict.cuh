@@ -57,14 +57,12 @@ struct Row {
     const int32_t *pos;
     int len, held, n_sink;
     int64_t shift, recent;  // positions >= recent are protected
-    __device__ __forceinline__ int64_t position(int i) const { return i < held ? (int64_t) pos[i] : i + shift; }
     __device__ __forceinline__ uint32_t key(int i) const {
-        const int64_t at = position(i);
-        if (at < n_sink || at >= recent) return 0xffffffffu;
-        const float a = acc[i];
-        if (a != a) return 0u;
+        const float a = acc[i];  // both loads at once
+        const int64_t at = i < held ? (int64_t) pos[i] : i + shift;
         const uint32_t u = __float_as_uint(a + 0.f);  // -0 + 0 = +0
-        return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+        const uint32_t k = a != a ? 0u : u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+        return at < n_sink || at >= recent ? 0xffffffffu : k;
     }
 };
 
@@ -76,33 +74,71 @@ __device__ __forceinline__ int row_len(const int32_t *seq_lens, int b, int max_l
     return 0;
 }
 
+// Exclusive scan of v over a block of kWarps warps (a row of warp totals in shared memory); *total gets
+// the sum.
+template <int kWarps>
 __device__ __forceinline__ int exclusive_scan(int v, int *warp_sums, int *total) {
-    return pages::block_exclusive_scan(v, warp_sums, total);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int w = lane < kWarps ? warp_sums[lane] : 0;  // every warp scans the totals for itself
+#pragma unroll
+    for (int off = 1; off < kWarps; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, w, off);
+        if (lane >= off) w += y;
+    }
+    *total = __shfl_sync(0xffffffffu, w, kWarps - 1);
+    const int before = warp > 0 ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
+    __syncthreads();  // warp_sums is reused by the next scan
+    return before + x - v;
 }
 
-// A row per cluster of C CTAs, each with a contiguous share of the row's keys. The budget-th largest
-// key is found digit by digit (11, 11 and 10 bits): shared-memory histograms of the keys that match the
-// digits found so far, summed over the cluster's CTAs through distributed shared memory, one array per
-// digit so that no CTA clears what another still reads. Then the ranks of equal keys, of holes and of
-// movers come from block scans plus the totals of the CTAs before. The weights and positions are read
-// once; the time is that of a dozen block and cluster barriers.
-__global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kMaxCluster = 8;
+
+// Counts of a stretch of keys against the threshold: above it and equal to it, below the budget's
+// index (low) and past it (high).
+struct Counts {
+    int gt_low, eq_low, gt_high, eq_high;
+    __device__ __forceinline__ void add(const Counts &o) {
+        gt_low += o.gt_low, eq_low += o.eq_low, gt_high += o.gt_high, eq_high += o.eq_high;
+    }
+};
+
+// A row per cluster of C CTAs, each with a contiguous share of the row's keys, and each warp with a
+// contiguous stretch of its CTA's. The budget-th largest key is found digit by digit (11, 11 and 10
+// bits): shared-memory histograms of the keys that match the digits found so far, summed over the
+// cluster's CTAs through distributed shared memory, one array per digit so that no CTA clears what
+// another still reads. The ranks of equal keys, of holes and of movers then come from ballots, the
+// warps' counts, and one exchange of the CTAs' counts (an equal key's rank decides whether it stays,
+// and equal keys in low indexes come before those in high ones, so the counts of kept keys follow
+// from Counts alone). The weights and positions are read once; the rest is latency: the
+// histograms' barriers, and the launch. 512 threads, so that two CTAs fit an SM and a GPC holds
+// several clusters of 8: with 1024 threads (one CTA per SM) 16 rows of 32768 keys took 52 us.
+__global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectParams p) {
     extern __shared__ uint32_t keys_s[];
-    __shared__ int hist[3][kBins];
-    __shared__ int warp_sums[32];
+    __shared__ __align__(16) int hist[3][kBins];  // read as int4
+    __shared__ int warp_sums[kSelectWarps];
     __shared__ int digit_s, before_s;
-    __shared__ int eq_total, hole_total, mover_total;
+    __shared__ Counts warp_counts[kSelectWarps], cta_counts;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
     const int b = blockIdx.x / C;
-    const int tid = threadIdx.x;
-    for (int i = tid; i < 3 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
     pdl_wait();
     pdl_launch_dependents();
     const int len = row_len(p.seq_lens, b, p.w.row_cells, p.status);
     int32_t *src = p.src + (int64_t) b * p.max_moves, *dst = p.dst + (int64_t) b * p.max_moves;
     if (len <= p.budget) {  // the whole cluster: nothing to evict
-        for (int j = rank * kThreads + tid; j < p.max_moves; j += C * kThreads) src[j] = dst[j] = -1;
+        for (int j = rank * kSelectThreads + tid; j < p.max_moves; j += C * kSelectThreads) src[j] = dst[j] = -1;
         if (rank == 0 && tid == 0) p.n_moves[b] = 0;
         return;
     }
@@ -116,9 +152,13 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
     row.recent = len + row.shift - p.n_recent;
     const int share = (len + C - 1) / C;
     const int first = min(rank * share, len), n = min(share, len - first);
+    const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
+    const int lo = min(warp * stretch, n), hi = min(lo + stretch, n);  // this warp's keys
     auto key = [&](int i) { return i < p.cap ? keys_s[i] : row.key(first + i); };
-    for (int i = tid; i < min(n, p.cap); i += kThreads) keys_s[i] = row.key(first + i);
-    __syncthreads();
+    // Each lane forms the keys it reads again below; eight steps' loads are in flight together (one step
+    // at a time, the two loads one after the other, cost 8 x 1.6 us of a 36 us pass over 4096 keys).
+#pragma unroll 8
+    for (int i = lo + lane; i < min(hi, p.cap); i += 32) keys_s[i] = row.key(first + i);
 
     uint32_t prefix = 0;
     int need = p.budget;  // keys still to be taken among those that match the prefix
@@ -126,25 +166,51 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
     for (int d = 0; d < 3; d++) {
         constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
         const int shift = kShift[d], bins = 1 << kBits[d];
-        for (int i = tid; i < n; i += kThreads) {
-            const uint32_t k = key(i);
-            if (d == 0 || (k >> (shift + kBits[d])) == prefix) atomicAdd(&hist[d][(k >> shift) & (bins - 1)], 1);
+        if (d == 0) __syncthreads();  // the histograms are clear
+        for (int i0 = lo; i0 < hi; i0 += 32) {
+            const int i = i0 + lane;
+            uint32_t k = 0;
+            bool in = i < hi;
+            if (in) {
+                k = key(i);
+                if (d > 0) in = (k >> (shift + kBits[d])) == prefix;
+            }
+            // the lanes that share the first lane's digit count as one (runs of protected tokens, of
+            // weights that are zero); the others one by one
+            const uint32_t live = __ballot_sync(0xffffffffu, in);
+            if (live == 0) continue;
+            const int bin = (int) ((k >> shift) & (uint32_t) (bins - 1));
+            const int lead = __ffs((int) live) - 1;
+            const int lead_bin = __shfl_sync(0xffffffffu, bin, lead);  // by every lane, whatever `in` is
+            const uint32_t same = __ballot_sync(0xffffffffu, in && bin == lead_bin);
+            if (lane == lead) atomicAdd(&hist[d][bin], __popc(same));
+            else if (in && !((same >> lane) & 1u)) atomicAdd(&hist[d][bin], 1);
         }
         cluster.sync();
-        // thread t: bins of descending digit, 2 t and 2 t + 1 from the top
-        int c[2] = {0, 0};
+        // thread t: four bins (two for the last digit) in descending order, 4 t .. 4 t + 3 from the top
+        constexpr int kPer[3] = {4, 4, 2};
+        int c[4] = {0, 0, 0, 0}, sum = 0;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int bin = bins - 1 - (2 * tid + e);
-            if (bin >= 0)
-                for (int r = 0; r < C; r++) c[e] += *cluster.map_shared_rank(&hist[d][bin], r);
+        for (int r = 0; r < kMaxCluster; r++) {
+            if (r < C) {
+                const int *h = cluster.map_shared_rank(&hist[d][0], r) + bins - kPer[d] * (tid + 1);
+                if (d < 2) {
+                    const int4 v = *reinterpret_cast<const int4 *>(h);
+                    c[0] += v.w, c[1] += v.z, c[2] += v.y, c[3] += v.x;
+                } else {
+                    const int2 v = *reinterpret_cast<const int2 *>(h);
+                    c[0] += v.y, c[1] += v.x;
+                }
+            }
         }
-        int total;
-        int above = exclusive_scan(c[0] + c[1], warp_sums, &total);
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < 4; e++) sum += c[e];
+        int total;
+        int above = exclusive_scan<kSelectWarps>(sum, warp_sums, &total);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
             if (above < need && need <= above + c[e]) {  // exactly one bin of the block
-                digit_s = bins - 1 - (2 * tid + e);
+                digit_s = bins - 1 - (kPer[d] * tid + e);
                 before_s = above;
             }
             above += c[e];
@@ -154,63 +220,82 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
         need -= before_s;
         __syncthreads();  // digit_s, before_s are written again
     }
-    // Kept: key > prefix, and the first `need` keys equal to it. Thread t walks `per` consecutive keys.
-    const int per = (n + kThreads - 1) / kThreads;
-    const int lo = min(tid * per, n), hi = min(lo + per, n);
-    int eq = 0;
-    for (int i = lo; i < hi; i++) eq += key(i) == prefix;
-    int total;
-    int eq_rank = exclusive_scan(eq, warp_sums, &total);
-    if (tid == 0) eq_total = total;
+    // Kept: key > prefix, and the first `need` keys equal to it.
+    const int edge = p.budget - first;  // indexes below it are low
+    Counts mine = {0, 0, 0, 0};
+    for (int i0 = lo; i0 < hi; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t k = i < hi ? key(i) : 0u;
+        const uint32_t gt = __ballot_sync(0xffffffffu, i < hi && k > prefix);
+        const uint32_t eq = __ballot_sync(0xffffffffu, i < hi && k == prefix);
+        const uint32_t low = __ballot_sync(0xffffffffu, i < edge);
+        mine.add({__popc(gt & low), __popc(eq & low), __popc(gt & ~low), __popc(eq & ~low)});
+    }
+    if (lane == 0) warp_counts[warp] = mine;
+    __syncthreads();
+    Counts before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kSelectWarps; w++) {
+        if (w == warp) before = all;
+        all.add(warp_counts[w]);
+    }
+    if (tid == 0) cta_counts = all;
     cluster.sync();
-    for (int r = 0; r < rank; r++) eq_rank += *cluster.map_shared_rank(&eq_total, r);
-    int holes = 0, movers = 0, rk = eq_rank;
-    for (int i = lo; i < hi; i++) {
-        const uint32_t k = key(i);
-        const bool kept = k > prefix || (k == prefix && rk++ < need);
-        if (first + i < p.budget) holes += !kept;
-        else movers += kept;
+    // eq keys, holes and movers of the CTAs before this one; all movers
+    int eq_at = 0, hole_at = 0, mover_at = 0, n_moves = 0, eq_seen = 0;
+    Counts other[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; r++)
+        if (r < C) other[r] = *cluster.map_shared_rank(&cta_counts, r);
+    cluster.sync();  // no CTA leaves while another reads its counts
+    auto kept_of = [&](int eq_before, int eq) { return max(0, min(eq, need - eq_before)); };
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; r++) {
+        if (r >= C) break;
+        const int r_first = min(r * share, len), r_end = r_first + min(share, len - r_first);
+        const int n_low = max(0, min(r_end, p.budget) - r_first);
+        const int kept_low = other[r].gt_low + kept_of(eq_seen, other[r].eq_low);
+        const int kept_high = other[r].gt_high + kept_of(eq_seen + other[r].eq_low, other[r].eq_high);
+        if (r == rank) eq_at = eq_seen, mover_at = n_moves;
+        if (r < rank) hole_at += n_low - kept_low;
+        eq_seen += other[r].eq_low + other[r].eq_high;
+        n_moves += kept_high;
     }
-    int hole_at = exclusive_scan(holes, warp_sums, &total);
-    if (tid == 0) hole_total = total;
-    int mover_at = exclusive_scan(movers, warp_sums, &total);
-    if (tid == 0) mover_total = total;
-    cluster.sync();
-    int n_moves = 0;
-    for (int r = 0; r < C; r++) {
-        const int m = *cluster.map_shared_rank(&mover_total, r);
-        if (r < rank) {
-            mover_at += m;
-            hole_at += *cluster.map_shared_rank(&hole_total, r);
-        }
-        n_moves += m;
+    // ... and of the warps before this one
+    {
+        const int n_low = max(0, min(lo, edge));
+        hole_at += n_low - before.gt_low - kept_of(eq_at, before.eq_low);
+        mover_at += before.gt_high + kept_of(eq_at + before.eq_low, before.eq_high);
+        eq_at += before.eq_low + before.eq_high;
     }
-    cluster.sync();  // no CTA leaves while another reads its totals
-    rk = eq_rank;
-    for (int i = lo; i < hi; i++) {
-        const uint32_t k = key(i);
-        const bool kept = k > prefix || (k == prefix && rk++ < need);
-        if (first + i < p.budget) {
-            if (!kept) dst[hole_at++] = first + i;
-        } else if (kept) {
-            src[mover_at++] = first + i;
-        }
+    const uint32_t lower = (1u << lane) - 1u;
+    for (int i0 = lo; i0 < hi; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t k = i < hi ? key(i) : 0u;
+        const uint32_t eq = __ballot_sync(0xffffffffu, i < hi && k == prefix);
+        const bool kept = i < hi && (k > prefix || (k == prefix && eq_at + __popc(eq & lower) < need));
+        const uint32_t hole = __ballot_sync(0xffffffffu, i < hi && i < edge && !kept);
+        const uint32_t mover = __ballot_sync(0xffffffffu, i >= edge && kept);
+        if ((hole >> lane) & 1u) dst[hole_at + __popc(hole & lower)] = first + i;
+        if ((mover >> lane) & 1u) src[mover_at + __popc(mover & lower)] = first + i;
+        eq_at += __popc(eq), hole_at += __popc(hole), mover_at += __popc(mover);
     }
-    for (int j = n_moves + rank * kThreads + tid; j < p.max_moves; j += C * kThreads) src[j] = dst[j] = -1;
+    for (int j = n_moves + rank * kSelectThreads + tid; j < p.max_moves; j += C * kSelectThreads) src[j] = dst[j] = -1;
     if (rank == 0 && tid == 0) p.n_moves[b] = n_moves;
 }
 
 // Planes whose rows (one cell each) a move copies: K and V, or the four planes of a q8_0 cache.
 struct MoveParams {
-    uint8_t *plane[4];
-    int row_bytes[4];  // multiples of 8; planes 0 and 1 of 16
-    int n_planes;
+    uint8_t *k, *v, *kd, *vd;
+    int row_bytes;    // of k and v, a multiple of 16
+    int small_bytes;  // of the scale planes, a multiple of 8; 0 = none
     const int32_t *block_tables;
     int n_rows, max_blocks;
     int64_t n_pages;
     const int32_t *n_moves;
     const int32_t *src, *dst;
     int max_moves;
+    int batch;  // moves of a warp, 1 .. 16
     DeviceStatus *status;
 };
 
@@ -230,32 +315,68 @@ __device__ __forceinline__ int64_t move_cell(const MoveParams &p, int b, int i) 
     return (int64_t) pid * pages::kBlock + i % pages::kBlock;
 }
 
-// A warp per move.
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveParams p) {
+// A warp takes `batch` consecutive moves of a row: its lanes look up all their cells at once, then the
+// moves are copied four at a time (16 bytes a lane, K and V together: 8 loads in flight), and the scale
+// planes with several moves to a pass.
+__device__ __forceinline__ void move_big(uint8_t *k, uint8_t *v, int bytes, int64_t cell, int count) {
+    const int lane = threadIdx.x & 31;
+    for (int m0 = 0; m0 < count; m0 += 4) {
+        int64_t from[4], to[4];
+        bool go[4];
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            from[m] = __shfl_sync(0xffffffffu, cell, (m0 + m) & 15) * bytes;
+            to[m] = __shfl_sync(0xffffffffu, cell, 16 + ((m0 + m) & 15)) * bytes;
+            go[m] = m0 + m < count && from[m] >= 0 && to[m] >= 0;
+        }
+        for (int o = lane * 16; o < bytes; o += 512) {
+            uint4 a[4], b[4];
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+                if (go[m]) {
+                    a[m] = *reinterpret_cast<const uint4 *>(k + from[m] + o);
+                    b[m] = *reinterpret_cast<const uint4 *>(v + from[m] + o);
+                }
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+                if (go[m]) {
+                    *reinterpret_cast<uint4 *>(k + to[m] + o) = a[m];
+                    *reinterpret_cast<uint4 *>(v + to[m] + o) = b[m];
+                }
+        }
+    }
+}
+__device__ __forceinline__ void move_small(uint8_t *k, uint8_t *v, int bytes, int64_t cell, int count) {
+    const int lane = threadIdx.x & 31, units = bytes / 8;  // 8-byte units of a row
+    for (int u0 = 0; u0 < count * units; u0 += 32) {
+        const int u = u0 + lane, m = min(u / units, 15);
+        const int64_t from = __shfl_sync(0xffffffffu, cell, m), to = __shfl_sync(0xffffffffu, cell, 16 + m);
+        if (u < count * units && from >= 0 && to >= 0) {
+            const int o = (u - m * units) * 8;
+            const uint2 a = *reinterpret_cast<const uint2 *>(k + from * bytes + o);
+            const uint2 b = *reinterpret_cast<const uint2 *>(v + from * bytes + o);
+            *reinterpret_cast<uint2 *>(k + to * bytes + o) = a;
+            *reinterpret_cast<uint2 *>(v + to * bytes + o) = b;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kMoveThreads, 3) move_kernel(const MoveParams p) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int64_t total = (int64_t) p.n_rows * p.max_moves;
+    const int64_t per_row = (p.max_moves + p.batch - 1) / p.batch, total = per_row * p.n_rows;
     for (int64_t x = (int64_t) blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); x < total;
          x += (int64_t) gridDim.x * (kMoveThreads / 32)) {
-        const int b = (int) (x / p.max_moves), j = (int) (x - (int64_t) b * p.max_moves);
-        if (j >= p.n_moves[b]) continue;
-        const int64_t from = move_cell(p, b, p.src[x]), to = move_cell(p, b, p.dst[x]);
-        if (from < 0 || to < 0) continue;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (k >= p.n_planes) break;
-            const int bytes = p.row_bytes[k];
-            const uint8_t *s = p.plane[k] + from * bytes;
-            uint8_t *d = p.plane[k] + to * bytes;
-            if (k < 2) {
-                for (int o = lane * 16; o < bytes; o += 512)
-                    *reinterpret_cast<uint4 *>(d + o) = *reinterpret_cast<const uint4 *>(s + o);
-            } else {
-                for (int o = lane * 8; o < bytes; o += 256)
-                    *reinterpret_cast<uint2 *>(d + o) = *reinterpret_cast<const uint2 *>(s + o);
-            }
-        }
+        const int b = (int) (x / per_row), j0 = (int) (x - (int64_t) b * per_row) * p.batch;
+        const int count = min(min(p.n_moves[b], p.max_moves) - j0, p.batch);
+        if (count <= 0) continue;
+        // lane m: the source cell of move j0 + m; lane 16 + m: its destination; -1 where out of range
+        const int m = lane & 15;
+        int64_t cell = -1;
+        if (m < count) cell = move_cell(p, b, (lane < 16 ? p.src : p.dst)[(int64_t) b * p.max_moves + j0 + m]);
+        move_big(p.k, p.v, p.row_bytes, cell, count);
+        if (p.small_bytes) move_small(p.kd, p.vd, p.small_bytes, cell, count);
     }
 }
 
@@ -317,7 +438,7 @@ __global__ void __launch_bounds__(kThreads) truncate_kernel(pages::State st, int
         const int len = tid < rows ? st.seq_lens[r0 + tid] : 0;
         const int freed = len > budget && len <= cells ? pages::n_blocks_for(len) - keep_blocks : 0;
         int total;
-        at_s[tid] = exclusive_scan(freed, warp_sums, &total);
+        at_s[tid] = exclusive_scan<kThreads / 32>(freed, warp_sums, &total);
         __syncthreads();
         for (int r = warp; r < rows; r += kThreads / 32) {
             const int l = st.seq_lens[r0 + r];

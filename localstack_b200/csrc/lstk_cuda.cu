@@ -1209,7 +1209,7 @@ int lstk_cuda_kv_evict_select(const lstk_kv_weights *weights, const int32_t *seq
     p.status = dev->status;
     // CTAs per row: one per 4096 cells, up to the portable cluster size of 8
     int cluster = 1;
-    while (cluster < 8 && (int64_t) cluster * 4096 < weights->row_cells) cluster *= 2;
+    while (cluster < evict::kMaxCluster && (int64_t) cluster * 4096 < weights->row_cells) cluster *= 2;
     p.cap = std::min((weights->row_cells + cluster - 1) / cluster, 32768);
     const size_t smem = sizeof(uint32_t) * (size_t) p.cap;
     if ((int64_t) weights->n_rows * cluster > (int64_t) INT32_MAX)
@@ -1218,7 +1218,7 @@ int lstk_cuda_kv_evict_select(const lstk_kv_weights *weights, const int32_t *seq
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) (weights->n_rows * cluster));
-    cfg.blockDim = dim3(evict::kThreads);
+    cfg.blockDim = dim3(evict::kSelectThreads);
     cfg.dynamicSmemBytes = smem;
     launch_pdl(cfg, attr, static_cast<cudaStream_t>(stream));
     attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -1237,7 +1237,7 @@ static int kv_move_impl(const char *fn, const lstk_kv_layout *layout, evict::Mov
         return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": NULL pointer");
     if (n_rows == 0 || max_moves == 0) return clear_error();
     DeviceInfo *dev = nullptr;
-    int rc = bind_device(p.plane[0], &dev);
+    int rc = bind_device(p.k, &dev);
     if (rc) return rc;
     p.block_tables = block_tables;
     p.n_rows = n_rows;
@@ -1250,7 +1250,11 @@ static int kv_move_impl(const char *fn, const lstk_kv_layout *layout, evict::Mov
     p.status = dev->status;
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = {};
-    const int64_t warps = (int64_t) n_rows * max_moves;
+    // Moves per warp: up to 16 (one round of lookups for all of them), fewer when that would leave SMs
+    // without warps.
+    p.batch = 16;
+    while (p.batch > 1 && (int64_t) n_rows * ((max_moves + p.batch - 1) / p.batch) < (int64_t) dev->n_sms * 32) p.batch /= 2;
+    const int64_t warps = (int64_t) n_rows * ((max_moves + p.batch - 1) / p.batch);
     cfg.gridDim = dim3((unsigned) std::min<int64_t>((warps + evict::kMoveThreads / 32 - 1) / (evict::kMoveThreads / 32),
                                                     (int64_t) dev->n_sms * 16));
     cfg.blockDim = dim3(evict::kMoveThreads);
@@ -1268,11 +1272,9 @@ int lstk_cuda_kv_move(const lstk_kv_layout *layout, void *k_cache, void *v_cache
     if (!aligned(k_cache, 16) || !aligned(v_cache, 16))
         return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": misaligned pointer");
     evict::MoveParams p = {};
-    const int row = layout->n_head_kv * layout->head_dim * 2;
-    p.plane[0] = static_cast<uint8_t *>(k_cache);
-    p.plane[1] = static_cast<uint8_t *>(v_cache);
-    p.row_bytes[0] = p.row_bytes[1] = row;
-    p.n_planes = 2;
+    p.k = static_cast<uint8_t *>(k_cache);
+    p.v = static_cast<uint8_t *>(v_cache);
+    p.row_bytes = layout->n_head_kv * layout->head_dim * 2;
     return kv_move_impl(fn, layout, p, block_tables, n_rows, max_blocks_per_seq, n_moves, move_src, move_dst, max_moves,
                         stream);
 }
@@ -1288,13 +1290,12 @@ int lstk_cuda_kv_move_q8(const lstk_kv_layout *layout, int8_t *k_qs, void *k_d, 
     if (!aligned(k_qs, 16) || !aligned(v_qs, 16) || !aligned(k_d, 8) || !aligned(v_d, 8))
         return set_error(LSTK_ERR_INVALID_ARG, std::string(fn) + ": misaligned plane");
     evict::MoveParams p = {};
-    p.plane[0] = reinterpret_cast<uint8_t *>(k_qs);
-    p.plane[1] = reinterpret_cast<uint8_t *>(v_qs);
-    p.plane[2] = static_cast<uint8_t *>(k_d);
-    p.plane[3] = static_cast<uint8_t *>(v_d);
-    p.row_bytes[0] = p.row_bytes[1] = layout->n_head_kv * layout->head_dim;
-    p.row_bytes[2] = p.row_bytes[3] = layout->n_head_kv * (layout->head_dim / 32) * 2;
-    p.n_planes = 4;
+    p.k = reinterpret_cast<uint8_t *>(k_qs);
+    p.v = reinterpret_cast<uint8_t *>(v_qs);
+    p.kd = static_cast<uint8_t *>(k_d);
+    p.vd = static_cast<uint8_t *>(v_d);
+    p.row_bytes = layout->n_head_kv * layout->head_dim;
+    p.small_bytes = layout->n_head_kv * (layout->head_dim / 32) * 2;
     return kv_move_impl(fn, layout, p, block_tables, n_rows, max_blocks_per_seq, n_moves, move_src, move_dst, max_moves,
                         stream);
 }
