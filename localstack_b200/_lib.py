@@ -159,6 +159,22 @@ def lib():
     return L
 
 
+_host_module = None
+
+
+def host():
+    """localstack_b200/_host.so: the bounded-cache wrappers' compiled calls (csrc/host_bind.cpp)."""
+    global _host_module
+    if _host_module is None:
+        lib()
+        try:
+            from . import _host
+        except ImportError as e:
+            raise FileNotFoundError(f"localstack_b200/_host.so is not built ({e}); run localstack_b200._lib.build()") from e
+        _host_module = _host
+    return _host_module
+
+
 def last_error():
     return lib().lstk_cuda_last_error().decode()
 

@@ -18,9 +18,8 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import KvWeightsState, check, lib
+from ._lib import KvWeightsState, check, host, lib
 from .attn import _p, _stream
-from .bounded import _caches, _planes
 from .q8 import Q8Cache
 
 BLOCK = 32
@@ -78,20 +77,13 @@ class KvWeights:
         n_recent stay, then the largest acc (lower index first among equal ones). Rows at or below the
         budget have none. `moves` (an earlier result for the same sizes) is written again if given."""
         budget = int(budget)
-        if seq_lens.dtype != torch.int32 or seq_lens.numel() != self.n_rows or not seq_lens.is_contiguous():
-            raise ValueError("seq_lens must be a contiguous int32 tensor, one per row")
-        most = max(0, min(budget, self.row_cells - budget))
+        given = (None, None, None) if moves is None else (moves.n, moves.src, moves.dst)
+        rc, n, src, dst = host().select(self.acc, self.pos, self.held, self.shift, seq_lens, budget, n_sink, n_recent,
+                                        *given, stream)
+        if rc:
+            check(rc)
         if moves is None:
-            room = torch.empty(self.n_rows * (2 * most + 1), dtype=torch.int32, device=self.device)
-            n, src, dst = room.split((self.n_rows, self.n_rows * most, self.n_rows * most))
-            moves = KvMoves(n, src.view(self.n_rows, most), dst.view(self.n_rows, most), budget)
-        elif (moves.src.shape != moves.dst.shape or moves.src.shape[0] != self.n_rows or moves.src.shape[1] < most
-              or moves.n.numel() != self.n_rows
-              or any(t.dtype != torch.int32 or not t.is_contiguous() for t in (moves.n, moves.src, moves.dst))):
-            raise ValueError("moves must hold min(budget, cells - budget) moves for every row")
-        check(lib().lstk_cuda_kv_evict_select(ctypes.byref(self.state), _p(seq_lens), budget, int(n_sink),
-                                              int(n_recent), moves.src.shape[1], _p(moves.n), _p(moves.src),
-                                              _p(moves.dst), _stream(stream, self.device)))
+            return KvMoves(n, src, dst, budget)
         moves.budget = budget
         return moves
 
@@ -116,22 +108,15 @@ class KvWeights:
         self.shift[slot].zero_()
 
 
-def _move(fn, layout, cache, device, block_tables, moves, stream):
-    rows = moves.src.shape[0]
-    if block_tables.dtype != torch.int32 or not block_tables.is_contiguous() or block_tables.dim() != 2 \
-            or block_tables.shape[0] != rows:
-        raise ValueError("block_tables must be a contiguous int32 [rows][max_blocks] tensor")
-    check(fn(ctypes.byref(layout), *cache, _p(block_tables), rows, block_tables.shape[1], _p(moves.n), _p(moves.src),
-             _p(moves.dst), moves.src.shape[1], _stream(stream, device)))
-
-
 def kv_move(k_cache, v_cache, block_tables, moves: KvMoves, stream=None):
     """Carries out an eviction's moves on one layer's K and V caches (f16 [n_cells][n_head_kv][128])."""
-    layout, cache, device = _caches(k_cache, v_cache)
-    _move(lib().lstk_cuda_kv_move, layout, cache, device, block_tables, moves, stream)
+    (rc,) = host().move(k_cache, None, v_cache, None, block_tables, moves.n, moves.src, moves.dst, stream)
+    if rc:
+        check(rc)
 
 
 def kv_move_q8(kq: Q8Cache, vq: Q8Cache, block_tables, moves: KvMoves, stream=None):
     """kv_move on q8_0 planes."""
-    layout, cache, device = _planes(kq, vq)
-    _move(lib().lstk_cuda_kv_move_q8, layout, cache, device, block_tables, moves, stream)
+    (rc,) = host().move(kq.qs, kq.d, vq.qs, vq.d, block_tables, moves.n, moves.src, moves.dst, stream)
+    if rc:
+        check(rc)
