@@ -417,8 +417,8 @@ int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, co
  * n_sink >= 0; a query that sees none gets zeros). Tiles between the sinks and the windows of a tile's
  * queries are neither read nor computed, and block_tables entries of pages that no query sees are
  * not looked at. out is f32 or bf16 (out_dtype; each f32 result rounded once). Cells that no query of
- * a 128-row tile sees may hold anything; a non-finite K or V value that one of them does see may reach
- * the tile's other rows. Other arguments, workspace and limits as lstk_cuda_attn_prefill; the _q8 form
+ * the 256 rows computed together sees may hold anything; a non-finite K or V value that one of them
+ * does see may reach the others. Other arguments, workspace and limits as lstk_cuda_attn_prefill; the _q8 form
  * as lstk_cuda_attn_prefill_q8 (same scratch), dequantising only the pages that some query sees. */
 int lstk_cuda_attn_prefill_window(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache,
                                   const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head,

@@ -11,6 +11,7 @@
 #include "kv_pages.cuh"
 #include "q8_layout.cuh"
 #include "prefill.cuh"
+#include "prefill_window.cuh"
 
 #include "lstk_cuda_attn.h"
 
@@ -894,7 +895,7 @@ size_t lstk_cuda_attn_prefill_workspace_size(int32_t n_seqs, int32_t n_head, int
     return align_up((size_t) total_tokens * n_head * head_dim * 2, 256);
 }
 
-// A prefill over a window with sinks (prefill.cuh's kWin).
+// A prefill over a window with sinks (prefill_window.cuh).
 struct PrefillWindow {
     const char *fn;
     int32_t window, n_sink, out_dtype;
@@ -968,19 +969,16 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
     CUtensorMap qmap, kmap, vmap, omap;
     const int tpt = prefill::kBM / group;
     if ((rc = encode_f16_3d(&qmap, q16, 128, n_head, total_tokens, 64, group, tpt))) return rc;
-    const bool out16 = pw && pw->out_dtype == LSTK_DTYPE_BF16;
-    if ((rc = out16 ? encode_3d(&omap, out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, 128, n_head, total_tokens, 64, group, tpt)
-                    : encode_f32_3d(&omap, out, 128, n_head, total_tokens, 32, group, tpt)))
-        return rc;
+    if (!pw && (rc = encode_f32_3d(&omap, out, 128, n_head, total_tokens, 32, group, tpt))) return rc;
     if ((rc = encode_f16_3d(&kmap, k_cache, 128, hkv, layout->n_cells, 64, 1, 32))) return rc;
     if ((rc = encode_f16_3d(&vmap, v_cache, 128, hkv, layout->n_cells, 64, 1, 32))) return rc;
 
-    prefill::Params p;
+    prefill_window::Params p;
     p.n_seqs = n_seqs;
     p.n_head = n_head;
     p.n_head_kv = hkv;
     p.group = group;
-    p.n_qt = (max_q_len + tpt - 1) / tpt;
+    p.n_qt = pw ? (max_q_len + 2 * tpt - 1) / (2 * tpt) : (max_q_len + tpt - 1) / tpt;  // a window's items are pairs
     p.total_tokens = (int) total_tokens;
     p.q_seq_start = q_seq_start;
     p.q_pos0 = q_pos0;
@@ -1001,23 +999,35 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
     p.n_items = (int) n_items;
     // Persistent: one CTA per SM walks its share of the items (snake order over heaviest-first).
     const int64_t grid = std::min<int64_t>(n_items, dev->n_sms);
-    const auto kernel = !pw     ? prefill::prefill_kernel<false, false>
-                        : out16 ? prefill::prefill_kernel<true, true>
-                                : prefill::prefill_kernel<true, false>;
-    if ((rc = ensure_smem(pw ? &dev->prefill_window_smem[out16] : &dev->prefill_smem, kernel, prefill::kSmemBytes,
-                          "cudaFuncSetAttribute(prefill)")))
-        return rc;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) grid);
+    if (pw) {
+        const bool out16 = pw->out_dtype == LSTK_DTYPE_BF16;
+        const auto kernel = out16 ? prefill_window::prefill_window_kernel<true> : prefill_window::prefill_window_kernel<false>;
+        if ((rc = ensure_smem(&dev->prefill_window_smem[out16], kernel, prefill_window::kSmemBytes,
+                              "cudaFuncSetAttribute(prefill window)")))
+            return rc;
+        cfg.blockDim = dim3(prefill_window::kThreads);
+        cfg.dynamicSmemBytes = prefill_window::kSmemBytes;
+        cfg.stream = s;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return launch_pdl_check(cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, p), "prefill_window_kernel");
+    }
+    if ((rc = ensure_smem(&dev->prefill_smem, prefill::prefill_kernel, prefill::kSmemBytes,
+                          "cudaFuncSetAttribute(prefill)")))
+        return rc;
     cfg.blockDim = dim3(prefill::kThreads);
     cfg.dynamicSmemBytes = prefill::kSmemBytes;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return launch_pdl_check(cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, omap, p), "prefill_kernel");
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg, prefill::prefill_kernel, qmap, kmap, vmap, omap,
+                                               static_cast<const prefill::Params &>(p)),
+                            "prefill_kernel");
 }
 
 int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,

@@ -56,15 +56,6 @@
 //   V: the B operand of PV with N = head dim contiguous ("MN-major"): sub-tile h holds dims
 //      64h..64h+63 of all 128 keys; LBO = 16 KiB between the two dim halves, SBO = 1 KiB
 //      between groups of 8 keys.
-//
-// Window with sinks (kWin). Query p sees keys i <= p with i > p - window or i < n_sink. An item's keys
-// are then the sinks' pages followed by the pages from its first query's window to its last query's
-// position; tiles are taken over that list of pages (Item::page), so pages between the two are neither
-// loaded nor multiplied, and each warp masks its two pages of a tile by a bit mask per row. Scores
-// of hidden keys are replaced, whatever K holds; V rows that no query of the item sees are cleared in
-// shared memory by the PV issuer's warp before they are multiplied (a cell outside the sequence or the
-// window may hold anything: 0 * inf is not 0). A non-finite V row that some query of the item does see
-// reaches the item's other rows, as in the plain kernel.
 #pragma once
 
 #include "common.cuh"
@@ -111,7 +102,6 @@ struct Params {
     DeviceStatus *status;
     uint64_t wait_ns;           // limit of each pipeline wait (drains keep kWaitLimitNs)
     const int32_t *start_flag;  // optional: the producers wait for it to be non-zero before loading
-    int window = 0, n_sink = 0;  // kWin
 };
 
 struct Barriers {
@@ -191,25 +181,7 @@ extern __shared__ __align__(1024) uint8_t dyn_smem[];
 struct Item {
     int b, kvh, tok0, q_begin, n_q, kv_len, pos0, n_keys, n_tiles;
     bool bad_rows;  // the sequence's query rows are not inside [0, total_tokens): no rows, reported
-    // kWin: the item's pages are n_sink_pages from page 0, then those from first_page on; n_pages in all
-    int n_sink_pages, first_page, n_pages;
-    int first;  // kWin: first key of the first query's window (at most n_keys)
-    __device__ __forceinline__ int page(int v) const { return v < n_sink_pages ? v : v - n_sink_pages + first_page; }
 };
-
-// Bit i: key i of page pg is at a position below n.
-__device__ __forceinline__ uint32_t below(int n, int pg) {
-    const int r = n - pg * kPage;
-    return r <= 0 ? 0u : r >= kPage ? 0xffffffffu : (1u << r) - 1u;
-}
-// First key of the window of the query at position pos (a window of up to 2^31 - 1 keys).
-__device__ __forceinline__ int window_first(int pos, int window) {
-    return (int) max((int64_t) 0, (int64_t) pos + 1 - window);
-}
-// Keys of page pg in [lo, hi) or below both n_sink and hi.
-__device__ __forceinline__ uint32_t window_mask(int pg, int lo, int hi, int n_sink) {
-    return below(hi, pg) & (~below(lo, pg) | below(n_sink, pg));
-}
 
 // An item's sequence metadata as loaded; item_finish derives the rest, so a loop can issue the
 // next item's loads early and use them one item later.
@@ -230,7 +202,6 @@ __device__ __forceinline__ ItemRaw item_load(const Params &p, int x) {
     return r;
 }
 
-template <bool kWin>
 __device__ __forceinline__ Item item_finish(const Params &p, const ItemRaw &r) {
     Item it;
     it.b = r.b;
@@ -246,21 +217,10 @@ __device__ __forceinline__ Item item_finish(const Params &p, const ItemRaw &r) {
     const int last_tok = min(it.tok0 + kBM / p.group, it.n_q) - 1;
     it.n_keys = it.tok0 < it.n_q ? max(0, min(it.kv_len, it.pos0 + last_tok + 1)) : 0;
     it.n_tiles = (it.n_keys + kBN - 1) / kBN;
-    if constexpr (kWin) {
-        const int end_page = (it.n_keys + kPage - 1) / kPage;
-        it.first = min(window_first(it.pos0 + it.tok0, p.window), it.n_keys);
-        it.first_page = it.first == it.n_keys ? end_page : it.first / kPage;
-        it.n_sink_pages = min((min(p.n_sink, it.first) + kPage - 1) / kPage, it.first_page);
-        it.n_pages = it.n_sink_pages + end_page - it.first_page;
-        it.n_tiles = (it.n_pages * kPage + kBN - 1) / kBN;
-    }
     return it;
 }
 
-template <bool kWin>
-__device__ __forceinline__ Item item_at(const Params &p, int x) {
-    return item_finish<kWin>(p, item_load(p, x));
-}
+__device__ __forceinline__ Item item_at(const Params &p, int x) { return item_finish(p, item_load(p, x)); }
 
 // The r-th item of this CTA (-1 past the end): rounds of gridDim.x items in "snake" order, forward
 // in even rounds and backward in odd ones, so the CTA that took one of the lightest items of a
@@ -271,8 +231,6 @@ __device__ __forceinline__ int item_index(const Params &p, int r) {
     return idx < p.n_items ? (int) idx : -1;
 }
 
-// kWin: window with sinks; kOut16: out is bf16, each f32 result rounded once.
-template <bool kWin, bool kOut16>
 __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ CUtensorMap qmap,
                                                               const __grid_constant__ CUtensorMap kmap,
                                                               const __grid_constant__ CUtensorMap vmap,
@@ -356,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         for (int r = 0; ok; r++) {
             const int x = item_index(p, r);
             if (x < 0) break;
-            const Item I = item_at<kWin>(p, x);
+            const Item I = item_at(p, x);
             if (I.n_tiles == 0) continue;
             if (is_k && lane == 0) {
                 if (n_items_t > 0)
@@ -372,12 +330,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             if (!ok) break;
             n_items_t++;
             const int32_t *bt = p.block_tables + (int64_t) I.b * p.max_blocks;
-            const int n_pg = kWin ? I.n_pages : (I.n_keys + kPage - 1) / kPage;  // pages holding visible keys
+            const int n_pg = (I.n_keys + kPage - 1) / kPage;  // pages holding visible keys
             auto load_chunk = [&](int chunk) -> int {
                 const int pi = chunk * 32 + lane;
                 int cell = (int) p.n_cells;  // out of bounds: TMA fills zeros
                 if (pi < n_pg) {
-                    const int32_t pid = bt[kWin ? I.page(pi) : pi];
+                    const int32_t pid = bt[pi];
                     if (pid >= 0 && pid < p.n_pages) cell = pid * kPage;
                     else if (is_k) report(p.status, kStatusBadIndex, kSitePrefillPage, pid);
                 }
@@ -445,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             for (int r = 0; ok; r++) {
                 const int x = item_index(p, r);
                 if (x < 0) break;
-                const int n = item_at<kWin>(p, x).n_tiles;
+                const int n = item_at(p, x).n_tiles;
                 if (n == 0) continue;
                 ok = mbar_wait_bounded(smem_u32(&bars->q_full), (uint32_t) n_items_t & 1, abort_flag, p.wait_ns);
                 for (int j = 0; ok && j < n; j++) {
@@ -485,58 +443,32 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     } else if (warp == kWarpMmaPv) {
         // ---- PV issuer: O_h += P_gg V_gg for key half h, as soon as that half's four softmax
         // warps have written P_gg; its commits (o_done, o_final) track only the PV MMAs. ----
-        // kWin: the whole warp walks the tiles (lane 0 issues), to clear hidden V rows.
-        if (kWin || lane == 0) {
+        if (lane == 0) {
             constexpr uint32_t idesc_pv = idesc_f16(true);
             const uint64_t dv0 = sdesc_sw128(sV, kSub, 1024);
             const uint32_t lv = (uint32_t) dv0;
             const uint64_t hv = dv0 & 0xFFFFFFFF00000000ull;
             int g = 0, n_items_t = 0;
             bool ok = true, issued = false;
-            auto wait = [&](uint64_t *bar, uint32_t parity) {
-                const bool done = mbar_wait_bounded(smem_u32(bar), parity, abort_flag, p.wait_ns);
-                return kWin ? __all_sync(0xffffffffu, done) : done;
-            };
             for (int r = 0; ok; r++) {
                 const int x = item_index(p, r);
                 if (x < 0) break;
-                const Item I = item_at<kWin>(p, x);
-                const int n = I.n_tiles;
+                const int n = item_at(p, x).n_tiles;
                 if (n == 0) continue;
                 for (int j = 0; ok && j < n; j++) {
                     const int gg = g + j;
                     const int buf = gg & 1;
-                    ok = wait(&bars->v_full[buf], (uint32_t) (gg >> 1) & 1);
-                    if constexpr (kWin) {
-                        if (!ok) break;
-                        bool cleared = false;
-                        for (int q = 0; q < 4; q++) {
-                            const int v = 4 * j + q;  // pages past the list are zeros already
-                            const uint32_t m = v < I.n_pages ? window_mask(I.page(v), I.first, I.n_keys, p.n_sink)
-                                                             : 0xffffffffu;
-                            if (m == 0xffffffffu) continue;
-                            cleared = true;
-                            // lane: 16 bytes of row pair member lane / 16, dim half (lane / 8) % 2
-                            uint8_t *page = base + kOffV + buf * kTile + ((lane >> 3) & 1) * kSub + q * (kPage * 128) +
-                                            (lane & 7) * 16;
-                            for (int r = lane >> 4; r < kPage; r += 2)
-                                if (!((m >> r) & 1u)) *reinterpret_cast<uint4 *>(page + r * 128) = make_uint4(0, 0, 0, 0);
-                        }
-                        if (cleared) {
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                    }
+                    ok = mbar_wait_bounded(smem_u32(&bars->v_full[buf]), (uint32_t) (gg >> 1) & 1, abort_flag, p.wait_ns);
                     // The item's first PV overwrites O: the previous item's epilogue must have read it.
                     if (ok && j == 0 && n_items_t > 0)
-                        ok = wait(&bars->o_free, (uint32_t) (n_items_t - 1) & 1);
+                        ok = mbar_wait_bounded(smem_u32(&bars->o_free), (uint32_t) (n_items_t - 1) & 1, abort_flag, p.wait_ns);
                     // P_gg sits in TMEM over S_gg: keys 0..63 in columns [0, 32), keys 64..127 in
                     // [64, 96) of the S buffer, two f16 per 32-bit column (16 keys per MMA step).
                     const uint32_t pcol = tmem + (buf ? kColS1 : kColS0);
                     for (int h = 0; h < 2 && ok; h++) {
-                        ok = wait(&bars->p_full[h][buf], (uint32_t) (gg >> 1) & 1);
+                        ok = mbar_wait_bounded(smem_u32(&bars->p_full[h][buf]), (uint32_t) (gg >> 1) & 1,
+                                               abort_flag, p.wait_ns);
                         if (!ok) break;
-                        if (kWin && lane != 0) continue;
                         tc_fence_after();
                         // V rows of K step kk: 16 keys x 128 B = 128 descriptor units from the tile start.
                         const uint32_t oc = tmem + (h ? kColO1 : kColO0), pc = pcol + (uint32_t) (h * 64);
@@ -547,14 +479,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                         issued = true;
                     }
                     if (!ok) break;
-                    if (kWin && lane != 0) continue;
                     mma_commit(smem_u32(&bars->o_done[buf]));
                     if (j == n - 1) mma_commit(smem_u32(&bars->o_final));
                 }
                 g += n;
                 n_items_t++;
             }
-            if (!ok && lane == 0) {
+            if (!ok) {
                 report(p.status, kStatusTimeout, kSitePrefillWait, kWarpMmaPv);
                 *abort_flag = 1;
             }
@@ -577,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         int x = item_index(p, 0);
         ItemRaw raw_next = x >= 0 ? item_load(p, x) : ItemRaw{};
         for (int it = 0; x >= 0; it++) {
-            const Item I = item_finish<kWin>(p, raw_next);
+            const Item I = item_finish(p, raw_next);
             if (I.bad_rows && warp == 0 && lane == 0) report(p.status, kStatusBadIndex, kSitePrefillRows, I.b);
             // The next item's metadata loads are issued now and used one item later.
             const int x_next = item_index(p, it + 1);
@@ -605,19 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 tmem_ld32(lane_base + (buf ? kColS1 : kColS0) + 64 * hf + 32, sc + 32);
                 tmem_wait_ld();
                 const int kbase = j * kBN + 64 * hf;  // key index of this warp's first column
-                if constexpr (kWin) {
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        const int v = 4 * j + 2 * hf + q;
-                        const int pg = I.page(v);  // past the list: at or past n_keys, so nothing is visible
-                        const uint32_t vis =
-                            v < I.n_pages ? window_mask(pg, window_first(I.pos0 + tq, p.window), row_keys, p.n_sink) : 0u;
-                        if (vis != 0xffffffffu) {
-#pragma unroll
-                            for (int c = 0; c < 32; c++) sc[32 * q + c] = (vis >> c) & 1u ? sc[32 * q + c] : -INFINITY;
-                        }
-                    }
-                } else if (kbase + 64 > row_keys) {
+                if (kbase + 64 > row_keys) {
 #pragma unroll
                     for (int c = 0; c < 64; c++) sc[c] = (kbase + c < row_keys) ? sc[c] : -INFINITY;
                 }
@@ -718,30 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     float o[32];
 #pragma unroll
                     for (int i = 0; i < 32; i++) o[i] = (use0 ? a[i] * c0 : 0.f) + (use1 ? b2[i] * c1 : 0.f);
-                    if constexpr (kOut16) {
-                        uint32_t w[16];  // bf16 pairs of these 32 columns
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const __nv_bfloat162 pr = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-                            w[i] = *reinterpret_cast<const uint32_t *>(&pr);
-                        }
-                        if (full && ok) {  // two 64-column boxes of 128 rows x 128 B
-                            const uint32_t box = sO + (uint32_t) hf * kSub;
-#pragma unroll
-                            for (int ch = 0; ch < 4; ch++)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                                 box + sw128_offset((uint32_t) r, (uint32_t) (4 * c + ch))),
-                                             "r"(w[4 * ch]), "r"(w[4 * ch + 1]), "r"(w[4 * ch + 2]), "r"(w[4 * ch + 3])
-                                             : "memory");
-                        } else if (!full && live && ok) {
-                            uint4 *dst = reinterpret_cast<uint4 *>(
-                                reinterpret_cast<__nv_bfloat16 *>(p.out) +
-                                ((int64_t) (I.q_begin + tq) * p.n_head + head) * kD + 64 * hf + 32 * c);
-#pragma unroll
-                            for (int ch = 0; ch < 4; ch++)
-                                dst[ch] = make_uint4(w[4 * ch], w[4 * ch + 1], w[4 * ch + 2], w[4 * ch + 3]);
-                        }
-                    } else if (full && ok) {
+                    if (full && ok) {
                         const uint32_t box = sO + (uint32_t) (2 * hf + c) * kSub;
 #pragma unroll
                         for (int ch = 0; ch < 8; ch++)
@@ -763,9 +659,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                     if (ok) fence_proxy_async_smem();
                     asm volatile("bar.sync 1, %0;" ::"r"(kSoftmaxWarps * 32) : "memory");
                     if (warp == 0 && lane == 0 && ok && !*abort_flag) {  // completes while the next item runs
-                        for (int bx = 0; bx < (kOut16 ? 2 : 4); bx++)
-                            tma_store_3d(&omap, sO + (uint32_t) bx * kSub, (kOut16 ? 64 : 32) * bx, I.kvh * G,
-                                         I.q_begin + I.tok0);
+                        for (int bx = 0; bx < 4; bx++)
+                            tma_store_3d(&omap, sO + (uint32_t) bx * kSub, 32 * bx, I.kvh * G, I.q_begin + I.tok0);
                         tma_store_commit();
                         store_pending = true;
                     }
@@ -774,17 +669,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                 n_items_t++;
             } else if (live) {
                 // no visible keys: the row's output is zero
-                if constexpr (kOut16) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) +
-                                                           ((int64_t) (I.q_begin + tq) * p.n_head + head) * kD + 64 * hf);
+                float *dst = p.out + ((int64_t) (I.q_begin + tq) * p.n_head + head) * kD + 64 * hf;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) dst[i] = make_uint4(0, 0, 0, 0);
-                } else {
-                    float *dst = p.out + ((int64_t) (I.q_begin + tq) * p.n_head + head) * kD + 64 * hf;
-#pragma unroll
-                    for (int i = 0; i < 64; i += 4)
-                        *reinterpret_cast<float4 *>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
-                }
+                for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             // All eight warps stop at the same item if any of them failed (every warp has run this
             // item's named barriers).

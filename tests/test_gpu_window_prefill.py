@@ -87,10 +87,13 @@ def test_rows_that_see_nothing_and_rows_of_no_sequence():
 
 
 def test_a_window_over_everything_is_attn_prefill():
+    """The two kernels take the row maxima over different key sets, so their roundings differ: both are
+    held to the exact result's bound, and hence to twice that bound of one another."""
     c = Chunks(RAGGED, 8, 2, seed=5)
     b = c.b
-    ref = L.attn_prefill(*b.cache, b.q, c.start_t, c.pos0_t, b.lens_t, b.bt, c.max_q)
-    assert torch.equal(c.run(1017, 0), ref) and torch.equal(c.run(2**31 - 1, 6), ref)
+    c.check(L.attn_prefill(*b.cache, b.q, c.start_t, c.pos0_t, b.lens_t, b.bt, c.max_q), 1017, 0)
+    c.check(c.run(1017, 0), 1017, 0)
+    assert torch.equal(c.run(1017, 0), c.run(2**31 - 1, 6))  # the same keys in the same tiles
 
 
 @pytest.mark.parametrize("q8", [False, True])
