@@ -30,7 +30,7 @@ namespace evict {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024;
-constexpr int kBins = 2048;
+constexpr int kBins = 256;  // 8 bits of a key at a time
 
 struct Weights {
     float *acc;      // [n_rows][row_cells]
@@ -102,39 +102,44 @@ __device__ __forceinline__ int exclusive_scan(int v, int *warp_sums, int *total)
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kShare = 8192;  // keys of a CTA before a row is split over more CTAs
 
 // Counts of a stretch of keys against the threshold: above it and equal to it, below the budget's
 // index (low) and past it (high).
-struct Counts {
+struct __align__(16) Counts {
     int gt_low, eq_low, gt_high, eq_high;
     __device__ __forceinline__ void add(const Counts &o) {
         gt_low += o.gt_low, eq_low += o.eq_low, gt_high += o.gt_high, eq_high += o.eq_high;
     }
 };
 
-// A row per cluster of C CTAs, each with a contiguous share of the row's keys, and each warp with a
-// contiguous stretch of its CTA's. The budget-th largest key is found digit by digit (11, 11 and 10
-// bits): shared-memory histograms of the keys that match the digits found so far, summed over the
-// cluster's CTAs through distributed shared memory, one array per digit so that no CTA clears what
-// another still reads. The ranks of equal keys, of holes and of movers then come from ballots, the
-// warps' counts, and one exchange of the CTAs' counts (an equal key's rank decides whether it stays,
-// and equal keys in low indexes come before those in high ones, so the counts of kept keys follow
-// from Counts alone). The weights and positions are read once; the rest is latency: the
-// histograms' barriers, and the launch. 512 threads, so that two CTAs fit an SM and a GPC holds
-// several clusters of 8: with 1024 threads (one CTA per SM) 16 rows of 32768 keys took 52 us.
+// A row per cluster of C CTAs (kMulti: C > 1), each with a contiguous share of the row's keys, and each
+// warp with a contiguous stretch of its CTA's. The budget-th largest key is found 8 bits at a time:
+// shared-memory histograms of the keys that match the bits found so far (one array per step, so that no
+// CTA clears what another still reads), copied once from the cluster's other CTAs (1 KiB each, through
+// distributed shared memory), and then every warp sums and scans the 256 bins for itself, without a
+// further barrier. The ranks of equal keys, of holes and of movers come from ballots, the warps' counts,
+// and one exchange of the CTAs' counts (an equal key's rank decides whether it stays, and equal keys in
+// low indexes come before those in high ones, so the counts of kept keys follow from Counts alone).
+// The weights and positions are read once; the rest is latency - a row of 544 keys takes PLACEHOLDER, 16
+// rows of up to 32768 PLACEHOLDER. Steps of 11 bits (three of 8 KiB) took 8.9 and 25.8 us: reading the
+// cluster's histograms cost more than the fourth step saves. 512 threads, so that two CTAs fit an SM and a
+// GPC holds several clusters of 8: with 1024 (one CTA per SM) the clusters ran one after the other.
+// The loops are kept rolled: code that runs once per launch costs its instruction fetches.
+template <bool kMulti>
 __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectParams p) {
     extern __shared__ uint32_t keys_s[];
-    __shared__ __align__(16) int hist[3][kBins];  // read as int4
-    __shared__ int warp_sums[kSelectWarps];
-    __shared__ int digit_s, before_s;
+    __shared__ __align__(16) int hist[4][kBins];  // read as int4
+    __shared__ __align__(16) int parts[kMulti ? kMaxCluster : 1][kBins];
     __shared__ Counts warp_counts[kSelectWarps], cta_counts;
     cg::cluster_group cluster = cg::this_cluster();
-    const int C = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
+    const int C = kMulti ? (int) cluster.num_blocks() : 1, rank = kMulti ? (int) cluster.block_rank() : 0;
     const int b = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int i = tid; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+    for (int i = tid; i < 4 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
     pdl_wait();
     pdl_launch_dependents();
+    const int held = p.w.held[b], shift_b = p.w.shift[b];  // in flight with the length
     const int len = row_len(p.seq_lens, b, p.w.row_cells, p.status);
     int32_t *src = p.src + (int64_t) b * p.max_moves, *dst = p.dst + (int64_t) b * p.max_moves;
     if (len <= p.budget) {  // the whole cluster: nothing to evict
@@ -146,91 +151,78 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
     row.acc = p.w.acc + (int64_t) b * p.w.row_cells;
     row.pos = p.w.pos + (int64_t) b * p.w.row_cells;
     row.len = len;
-    row.held = min(max(p.w.held[b], 0), len);
+    row.held = min(max(held, 0), len);
     row.n_sink = p.n_sink;
-    row.shift = p.w.shift[b];
+    row.shift = shift_b;
     row.recent = len + row.shift - p.n_recent;
     const int share = (len + C - 1) / C;
     const int first = min(rank * share, len), n = min(share, len - first);
     const int stretch = ((n + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
     const int lo = min(warp * stretch, n), hi = min(lo + stretch, n);  // this warp's keys
-    auto key = [&](int i) { return i < p.cap ? keys_s[i] : row.key(first + i); };
-    // Each lane forms the keys it reads again below; eight steps' loads are in flight together (one step
-    // at a time, the two loads one after the other, cost 8 x 1.6 us of a 36 us pass over 4096 keys).
-#pragma unroll 8
+    // Each lane forms the keys it reads again below (those beyond cap again at each use).
+#pragma unroll 4
     for (int i = lo + lane; i < min(hi, p.cap); i += 32) keys_s[i] = row.key(first + i);
+    const bool cached = hi <= p.cap;
+    auto key = [&](int i) { return cached || i < p.cap ? keys_s[i] : row.key(first + i); };
 
     uint32_t prefix = 0;
     int need = p.budget;  // keys still to be taken among those that match the prefix
-#pragma unroll
-    for (int d = 0; d < 3; d++) {
-        constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
-        const int shift = kShift[d], bins = 1 << kBits[d];
-        if (d == 0) __syncthreads();  // the histograms are clear
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            uint32_t k = 0;
-            bool in = i < hi;
-            if (in) {
-                k = key(i);
-                if (d > 0) in = (k >> (shift + kBits[d])) == prefix;
-            }
-            // the lanes that share the first lane's digit count as one (runs of protected tokens, of
-            // weights that are zero); the others one by one
-            const uint32_t live = __ballot_sync(0xffffffffu, in);
-            if (live == 0) continue;
-            const int bin = (int) ((k >> shift) & (uint32_t) (bins - 1));
-            const int lead = __ffs((int) live) - 1;
-            const int lead_bin = __shfl_sync(0xffffffffu, bin, lead);  // by every lane, whatever `in` is
-            const uint32_t same = __ballot_sync(0xffffffffu, in && bin == lead_bin);
-            if (lane == lead) atomicAdd(&hist[d][bin], __popc(same));
-            else if (in && !((same >> lane) & 1u)) atomicAdd(&hist[d][bin], 1);
+    __syncthreads();      // the histograms are clear
+#pragma unroll 1
+    for (int d = 0; d < 4; d++) {
+        const int shift = 24 - 8 * d;
+        // One shared-memory atomic per key: runs of equal keys (protected tokens, weights of zero) conflict,
+        // which costs less than aggregating them would for all the others.
+        for (int i = lo + lane; i < hi; i += 32) {
+            const uint32_t k = key(i);
+            if (d == 0 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[d][(k >> shift) & (kBins - 1)], 1);
         }
-        cluster.sync();
-        // thread t: four bins (two for the last digit) in descending order, 4 t .. 4 t + 3 from the top
-        constexpr int kPer[3] = {4, 4, 2};
-        int c[4] = {0, 0, 0, 0}, sum = 0;
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; r++) {
-            if (r < C) {
-                const int *h = cluster.map_shared_rank(&hist[d][0], r) + bins - kPer[d] * (tid + 1);
-                if (d < 2) {
-                    const int4 v = *reinterpret_cast<const int4 *>(h);
-                    c[0] += v.w, c[1] += v.z, c[2] += v.y, c[3] += v.x;
-                } else {
-                    const int2 v = *reinterpret_cast<const int2 *>(h);
-                    c[0] += v.y, c[1] += v.x;
-                }
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) sum += c[e];
-        int total;
-        int above = exclusive_scan<kSelectWarps>(sum, warp_sums, &total);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (above < need && need <= above + c[e]) {  // exactly one bin of the block
-                digit_s = bins - 1 - (kPer[d] * tid + e);
-                before_s = above;
-            }
-            above += c[e];
+        if constexpr (kMulti) {
+            cluster.sync();
+            // thread t: four bins of CTA t / 64
+            const int r = tid >> 6, q = tid & 63;
+            if (r < C) reinterpret_cast<int4 *>(parts[r])[q] = reinterpret_cast<const int4 *>(cluster.map_shared_rank(&hist[d][0], r))[q];
         }
         __syncthreads();
-        prefix = (prefix << kBits[d]) | (uint32_t) digit_s;
-        need -= before_s;
-        __syncthreads();  // digit_s, before_s are written again
+        // lane l: bins 255 - 8 l down to 248 - 8 l
+        int c[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0;
+#pragma unroll
+        for (int r = 0; r < (kMulti ? kMaxCluster : 1); r++) {
+            if (kMulti && r >= C) break;
+            const int4 *h = reinterpret_cast<const int4 *>(kMulti ? parts[r] : hist[d]) + 2 * (31 - lane);
+            const int4 u = h[0], v = h[1];
+            c[0] += v.w, c[1] += v.z, c[2] += v.y, c[3] += v.x, c[4] += u.w, c[5] += u.z, c[6] += u.y, c[7] += u.x;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum += c[e];
+        int above = sum;  // of the bins over this lane's
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, above, off);
+            if (lane >= off) above += y;
+        }
+        above -= sum;
+        const uint32_t has = __ballot_sync(0xffffffffu, above < need && need <= above + sum);  // exactly one lane
+        int digit = 255 - 8 * lane;
+#pragma unroll
+        for (int e = 0; e < 7; e++) {
+            if (need > above + c[e] && digit == 255 - 8 * lane - e) above += c[e], digit--;
+        }
+        const int from = __ffs((int) has) - 1;
+        prefix = (prefix << 8) | (uint32_t) __shfl_sync(0xffffffffu, digit, from);
+        need -= __shfl_sync(0xffffffffu, above, from);
     }
     // Kept: key > prefix, and the first `need` keys equal to it.
     const int edge = p.budget - first;  // indexes below it are low
     Counts mine = {0, 0, 0, 0};
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t k = i < hi ? key(i) : 0u;
-        const uint32_t gt = __ballot_sync(0xffffffffu, i < hi && k > prefix);
-        const uint32_t eq = __ballot_sync(0xffffffffu, i < hi && k == prefix);
-        const uint32_t low = __ballot_sync(0xffffffffu, i < edge);
-        mine.add({__popc(gt & low), __popc(eq & low), __popc(gt & ~low), __popc(eq & ~low)});
+    for (int i = lo + lane; i < hi; i += 32) {
+        const uint32_t k = key(i);
+        const int gt = k > prefix, eq = k == prefix;
+        if (i < edge) mine.gt_low += gt, mine.eq_low += eq;
+        else mine.gt_high += gt, mine.eq_high += eq;
     }
+    mine = {__reduce_add_sync(0xffffffffu, mine.gt_low), __reduce_add_sync(0xffffffffu, mine.eq_low),
+            __reduce_add_sync(0xffffffffu, mine.gt_high), __reduce_add_sync(0xffffffffu, mine.eq_high)};
     if (lane == 0) warp_counts[warp] = mine;
     __syncthreads();
     Counts before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
@@ -239,18 +231,26 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
         if (w == warp) before = all;
         all.add(warp_counts[w]);
     }
-    if (tid == 0) cta_counts = all;
-    cluster.sync();
+    if (kMulti) {
+        if (tid == 0) cta_counts = all;
+        cluster.sync();
+    }
     // eq keys, holes and movers of the CTAs before this one; all movers
     int eq_at = 0, hole_at = 0, mover_at = 0, n_moves = 0, eq_seen = 0;
-    Counts other[kMaxCluster];
+    Counts other[kMulti ? kMaxCluster : 1];
+    if constexpr (kMulti) {
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; r++)
-        if (r < C) other[r] = *cluster.map_shared_rank(&cta_counts, r);
-    cluster.sync();  // no CTA leaves while another reads its counts
+        for (int r = 0; r < kMaxCluster; r++)
+            if (r < C) other[r] = *cluster.map_shared_rank(&cta_counts, r);
+        // Waited for at the end: no CTA leaves while another reads its counts. (The arrival orders the
+        // loads above before it.)
+        cluster.barrier_arrive();
+    } else {
+        other[0] = all;
+    }
     auto kept_of = [&](int eq_before, int eq) { return max(0, min(eq, need - eq_before)); };
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; r++) {
+    for (int r = 0; r < (kMulti ? kMaxCluster : 1); r++) {
         if (r >= C) break;
         const int r_first = min(r * share, len), r_end = r_first + min(share, len - r_first);
         const int n_low = max(0, min(r_end, p.budget) - r_first);
@@ -269,19 +269,32 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
         eq_at += before.eq_low + before.eq_high;
     }
     const uint32_t lower = (1u << lane) - 1u;
+    const bool some_eq = mine.eq_low + mine.eq_high > 0;
     for (int i0 = lo; i0 < hi; i0 += 32) {
         const int i = i0 + lane;
         const uint32_t k = i < hi ? key(i) : 0u;
-        const uint32_t eq = __ballot_sync(0xffffffffu, i < hi && k == prefix);
-        const bool kept = i < hi && (k > prefix || (k == prefix && eq_at + __popc(eq & lower) < need));
-        const uint32_t hole = __ballot_sync(0xffffffffu, i < hi && i < edge && !kept);
-        const uint32_t mover = __ballot_sync(0xffffffffu, i >= edge && kept);
-        if ((hole >> lane) & 1u) dst[hole_at + __popc(hole & lower)] = first + i;
-        if ((mover >> lane) & 1u) src[mover_at + __popc(mover & lower)] = first + i;
-        eq_at += __popc(eq), hole_at += __popc(hole), mover_at += __popc(mover);
+        bool kept = k > prefix;
+        if (some_eq) {
+            const uint32_t eq = __ballot_sync(0xffffffffu, i < hi && k == prefix);
+            kept = kept || (k == prefix && eq_at + __popc(eq & lower) < need);
+            eq_at += __popc(eq);
+        }
+        if (i0 < edge) {
+            const bool hole = i < hi && i < edge && !kept;
+            const uint32_t holes = __ballot_sync(0xffffffffu, hole);
+            if (hole) dst[hole_at + __popc(holes & lower)] = first + i;
+            hole_at += __popc(holes);
+        }
+        if (i0 + 32 > edge) {
+            const bool mover = i < hi && i >= edge && kept;
+            const uint32_t movers = __ballot_sync(0xffffffffu, mover);
+            if (mover) src[mover_at + __popc(movers & lower)] = first + i;
+            mover_at += __popc(movers);
+        }
     }
     for (int j = n_moves + rank * kSelectThreads + tid; j < p.max_moves; j += C * kSelectThreads) src[j] = dst[j] = -1;
     if (rank == 0 && tid == 0) p.n_moves[b] = n_moves;
+    if constexpr (kMulti) cluster.barrier_wait();
 }
 
 // Planes whose rows (one cell each) a move copies: K and V, or the four planes of a q8_0 cache.

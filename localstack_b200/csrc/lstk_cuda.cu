@@ -42,7 +42,7 @@ struct DeviceInfo {
     size_t prefill_window_smem[2] = {};  // per out_dtype (f32, bf16)
     size_t append_smem[8] = {};  // per kv_append instantiation (append_kernel)
     size_t gemm_smem = 0;
-    size_t evict_smem = 0;
+    size_t evict_smem[2] = {};  // per select_kernel instantiation (one CTA per row, a cluster)
     // Resident kv_append CTAs per SM, per [instantiation][rows per group / 4]; 0 = not asked yet.
     int append_occ[8][append::kMaxGroupRows / 4 + 1] = {};
 };
@@ -1217,14 +1217,15 @@ int lstk_cuda_kv_evict_select(const lstk_kv_weights *weights, const int32_t *seq
     p.src = move_src;
     p.dst = move_dst;
     p.status = dev->status;
-    // CTAs per row: one per 4096 cells, up to the portable cluster size of 8
+    // CTAs per row: one per kShare cells, up to the portable cluster size
     int cluster = 1;
-    while (cluster < evict::kMaxCluster && (int64_t) cluster * 4096 < weights->row_cells) cluster *= 2;
-    p.cap = std::min((weights->row_cells + cluster - 1) / cluster, 32768);
+    while (cluster < evict::kMaxCluster && (int64_t) cluster * evict::kShare < weights->row_cells) cluster *= 2;
+    p.cap = std::min(((weights->row_cells + cluster - 1) / cluster + 31) / 32 * 32, 32768);
     const size_t smem = sizeof(uint32_t) * (size_t) p.cap;
     if ((int64_t) weights->n_rows * cluster > (int64_t) INT32_MAX)
         return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": too many rows");
-    if ((rc = ensure_smem(&dev->evict_smem, evict::select_kernel, smem, "cudaFuncSetAttribute(evict)"))) return rc;
+    const auto kernel = cluster > 1 ? evict::select_kernel<true> : evict::select_kernel<false>;
+    if ((rc = ensure_smem(&dev->evict_smem[cluster > 1], kernel, smem, "cudaFuncSetAttribute(evict)"))) return rc;
     cudaLaunchAttribute attr[2];
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) (weights->n_rows * cluster));
@@ -1235,7 +1236,7 @@ int lstk_cuda_kv_evict_select(const lstk_kv_weights *weights, const int32_t *seq
     attr[1].val.clusterDim.x = (unsigned) cluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
-    return launch_pdl_check(cudaLaunchKernelEx(&cfg, evict::select_kernel, p), "evict select_kernel");
+    return launch_pdl_check(cudaLaunchKernelEx(&cfg, kernel, p), "evict select_kernel");
 }
 
 static int kv_move_impl(const char *fn, const lstk_kv_layout *layout, evict::MoveParams &p, const int32_t *block_tables,
