@@ -978,6 +978,7 @@ struct CombineParams {
     float *out;
     float *lse_out;
     int out_bf16;  // out is bf16 (the kernels instantiated for a typed output only)
+    int early;     // kWeights: let the accumulation be scheduled now (it waits for this grid)
     // Exchange across ranks (decode_combine_kernel<true>): the mailboxes of the exchange-merge
     // protocol (exchange.cuh) for n_seqs * n_head rows, this rank, the rank count, the flag-wait
     // bound and the device status.
@@ -1171,6 +1172,7 @@ __device__ __forceinline__ void merge_state(float &m, float &den, float4 &acc, f
 template <bool kExchange, bool kTyped = false>
 __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(const CombineParams p) {
     pdl_wait();  // the split grid's partials and prefix are complete and visible
+    if (p.early) pdl_launch_dependents();
     const int S = p.dsplit;
     const int b = blockIdx.x, hg = blockIdx.y;
     const int zr = blockIdx.z / S, q = blockIdx.z - zr * S;
@@ -1335,6 +1337,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
 template <bool kTyped>
 __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_rows_kernel(const CombineParams p) {
     pdl_wait();  // the split grid's partials and prefix are complete and visible
+    if (p.early) pdl_launch_dependents();
     const int b = blockIdx.x, hg = blockIdx.y, w = blockIdx.z;
     const int kvh = hg * kHeadsPerGroup + w;
     if (kvh >= p.n_head_kv) return;
@@ -1435,8 +1438,9 @@ struct AccumulateParams {
 };
 
 constexpr int kAccumulateThreads = 256;
+constexpr int kAccumulateCtas = 6;  // per SM, all resident: each warp has one stretch of pages
 
-__global__ void __launch_bounds__(kAccumulateThreads) weights_accumulate_kernel(const AccumulateParams p) {
+__global__ void __launch_bounds__(kAccumulateThreads, kAccumulateCtas) weights_accumulate_kernel(const AccumulateParams p) {
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int n_pages = p.prefix[p.n_seqs];

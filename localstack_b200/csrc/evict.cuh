@@ -99,7 +99,7 @@ __device__ __forceinline__ int exclusive_scan(int v, int *warp_sums, int *total)
     return before + x - v;
 }
 
-constexpr int kSelectThreads = 512;
+constexpr int kSelectThreads = 1024;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kShare = 8192;  // keys of a CTA before a row is split over more CTAs
@@ -127,7 +127,7 @@ struct __align__(16) Counts {
 // GPC holds several clusters of 8: with 1024 (one CTA per SM) the clusters ran one after the other.
 // The loops are kept rolled: code that runs once per launch costs its instruction fetches.
 template <bool kMulti>
-__global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const SelectParams p) {
     extern __shared__ uint32_t keys_s[];
     __shared__ __align__(16) int hist[4][kBins];  // read as int4
     __shared__ __align__(16) int parts[kMulti ? kMaxCluster : 1][kBins];

@@ -494,6 +494,7 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
     c.out = p.out;
     c.lse_out = p.lse_out;
     c.out_bf16 = p.out_bf16;
+    c.early = mode == decode::kWeights;
     c.mailboxes = ex ? ex->mailboxes : nullptr;
     c.rank = ex ? ex->rank : 0;
     c.n_ranks = ex ? ex->n_ranks : 1;
@@ -708,7 +709,7 @@ static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) std::max<int64_t>(
-        1, std::min<int64_t>((n_seqs * max_pages + kPagesPerCta - 1) / kPagesPerCta, (int64_t) dev->n_sms * 8)));
+        1, std::min<int64_t>((n_seqs * max_pages + kPagesPerCta - 1) / kPagesPerCta, (int64_t) dev->n_sms * decode::kAccumulateCtas)));
     cfg.blockDim = dim3(decode::kAccumulateThreads);
     launch_pdl(cfg, attr, static_cast<cudaStream_t>(stream));
     return launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::weights_accumulate_kernel, a), "weights_accumulate_kernel");
