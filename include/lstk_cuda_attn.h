@@ -276,10 +276,14 @@ int lstk_cuda_kv_release(const lstk_kv_pages *state, int32_t slot, int32_t keep,
  *      row's moves; max_moves >= min(budget, row_cells - budget). Changes nothing else. A row's keys
  *      must not exceed row_cells (else it is reported, with no moves). n_sink + n_recent <= budget.
  *   2. lstk_cuda_kv_move (or _q8) for each layer's cache: copies the moved rows of K and V through the
- *      block tables. A move whose index or page is out of range is skipped and reported.
+ *      block tables. A move whose index or page is out of range is skipped and reported. The moves of a
+ *      call are carried out in no order: no cell may be the source of one and the destination of another
+ *      (select's never are).
  *   3. lstk_cuda_kv_evict_finish: moves acc and pos, clears acc behind the budget, advances held and
  *      shift, and truncates the rows to budget (KvCache::truncate_seq in row order,
  *      src/kv_cache.cpp:85-132: their blocks return to the free stack).
+ * Between 1 and 3 no token is appended to a row (the moves name the keys that select saw; a later one past
+ * the budget would be dropped).
  * The kept keys are then in no particular order, which decode attention does not see; a window
  * (lstk_cuda_attn_decode_window) is taken over positions and does not apply to such a row. Set the
  * row of a removed sequence back to zero (acc, held, shift) before its slot is used again. */

@@ -211,6 +211,7 @@ PyObject *window(PyObject *const *a) {
     same_device(c.k, ws);
     OnStream s(a[17], c.k.device());
     d.allocate();
+    if (d.B == 0) return result(LSTK_OK, d.out, d.lse);
     const size_t need = lstk_cuda_attn_decode_workspace_size(d.B, d.Hq, c.layout.n_head_kv, (int32_t) kD);
     if (bytes(ws) < need) ws = scratch(need, d.q);
     const int rc =
@@ -250,6 +251,7 @@ PyObject *weights(PyObject *const *a) {
     same_device(c.k, ws);
     OnStream s(a[16], c.k.device());
     d.allocate();
+    if (d.B == 0) return result(LSTK_OK, d.out, d.lse);
     if (!ws.defined())
         ws = scratch(lstk_cuda_attn_decode_weights_workspace_size(d.B, d.Hq, c.layout.n_head_kv, (int32_t) kD, (int32_t) max_len),
                      d.q);
@@ -300,6 +302,7 @@ PyObject *prefill(PyObject *const *a) {
     for (const at::Tensor *t : Tensors{&c.kd, &c.v, &c.vd, &q, &i[0], &i[1], &i[2], &i[3], &out, &ws, &sc}) same_device(c.k, *t);
     OnStream s(a[17], c.k.device());
     if (!out.defined()) out = at::empty(q.sizes(), q.options().dtype(type));
+    if (B == 0 || q.size(0) == 0) return result(LSTK_OK, out);
     const int32_t Hq = (int32_t) q.size(1), hkv = c.layout.n_head_kv;
     const size_t need = lstk_cuda_attn_prefill_workspace_size((int32_t) B, Hq, hkv, (int32_t) kD, max_q, max_blocks,
                                                               q.size(0), dtype_of(q));
@@ -352,6 +355,7 @@ PyObject *select(PyObject *const *a) {
         src = at::empty({rows, most}, lens.options());
         dst = at::empty({rows, most}, lens.options());
     }
+    if (rows == 0) return result(LSTK_OK, n, src, dst);
     const lstk_kv_weights w = {static_cast<float *>(ptr(acc)), static_cast<int32_t *>(ptr(pos)),
                                static_cast<int32_t *>(ptr(held)), static_cast<int32_t *>(ptr(shift)), (int32_t) rows,
                                (int32_t) cells};
@@ -373,6 +377,7 @@ PyObject *move(PyObject *const *a) {
     require(src.size(0) <= INT32_MAX && src.size(1) <= INT32_MAX && tables.size(1) <= INT32_MAX, "sizes out of range");
     for (const at::Tensor *t : Tensors{&c.kd, &c.v, &c.vd, &tables, &n, &src, &dst}) same_device(c.k, *t);
     OnStream s(a[8], c.k.device());
+    if (src.size(0) == 0 || src.size(1) == 0) return result(LSTK_OK);
     const int32_t rows = (int32_t) src.size(0), cap = (int32_t) src.size(1), max_blocks = (int32_t) tables.size(1);
     const int32_t *bt = static_cast<int32_t *>(ptr(tables)), *np = static_cast<int32_t *>(ptr(n));
     const int32_t *sp = static_cast<int32_t *>(ptr(src)), *dp = static_cast<int32_t *>(ptr(dst));

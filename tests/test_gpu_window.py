@@ -138,3 +138,116 @@ def test_stream_graph_and_moving_lengths():
         _check(b, out, lse, window, n_sink)
         o, _, _, t, _, _ = c.decode_ref(0, 99, 1)
         close(out_c.cpu().numpy(), o, t)
+
+
+def _policy(wait_ns, flag):
+    _lib.check(L.lib().lstk_cuda_set_wait_policy(int(wait_ns), None if flag is None else flag.data_ptr()))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("op", ["window", "weights", "prefill"])
+def test_a_wait_that_runs_out_is_reported_and_the_context_stays_usable(op, q8):
+    """The loaders are gated on a flag that nothing sets, with a limit of 2 ms (host-visible status, no
+    fault): LSTK_ERR_TIMEOUT, and the next call is right."""
+    b = Batch([4000, 33, 1, 700], 32, 4, seed=12, q8=q8)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    acc = torch.zeros(4, b.bt.shape[1] * 32, device="cuda")
+    sfx = "_q8" if q8 else ""
+
+    def call():
+        if op == "window":
+            return getattr(L, "attn_decode_window" + sfx)(*b.cache, b.q, b.bt, b.lens_t, 300, 4)
+        if op == "weights":
+            return getattr(L, "attn_decode_weights" + sfx)(*b.cache, b.q, b.bt, b.lens_t, acc)
+        return getattr(L, "attn_prefill_window" + sfx)(*b.cache, b.q, i32([0, 1, 2, 3, 4]), b.lens_t - 1, b.lens_t, b.bt, 1,
+                                                       300, 4)
+
+    want = call()
+    L.check_status()
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _policy(2_000_000, flag)
+    try:
+        call()
+        with pytest.raises(L.LstkError) as e:
+            L.check_status()
+        assert e.value.code == _lib.LSTK_ERR_TIMEOUT
+        flag.fill_(1)  # a gate that is open changes nothing
+        _policy(500_000_000, flag)
+        acc.zero_()
+        assert torch.equal(call(), want)
+        L.check_status()
+    finally:
+        _policy(0, None)
+    acc.zero_()
+    assert torch.equal(call(), want)
+    L.check_status()
+
+
+def test_streams_given_by_the_caller():
+    """A call on another stream than the current one: its outputs and scratch belong to that stream, and the
+    current stream and device are as before."""
+    b = Batch([900, 64], 32, 4, seed=13, q_dtype=torch.float32)
+    side = torch.cuda.Stream()
+    acc, acc2 = (torch.zeros(2, b.bt.shape[1] * 32, device="cuda") for _ in range(2))
+    start, pos0 = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), b.lens_t - 1
+    torch.cuda.synchronize()
+    results = []
+    for stream in (None, side):
+        before = torch.cuda.current_stream()
+        results.append((L.attn_decode_window(*b.cache, b.q, b.bt, b.lens_t, 70, 3, stream=stream),
+                        L.attn_decode_weights(*b.cache, b.q, b.bt, b.lens_t, acc if stream is None else acc2, stream=stream),
+                        L.attn_prefill_window(*b.cache, b.q, start, pos0, b.lens_t, b.bt, 1, 70, 3, stream=stream)))
+        assert torch.cuda.current_stream() == before and torch.cuda.current_device() == 0
+        torch.cuda.synchronize()
+    L.check_status()
+    assert all(torch.equal(x, y) for x, y in zip(*results)) and torch.equal(acc, acc2)
+
+
+def test_empty_calls():
+    b = Batch([40], 16, 8, seed=14)
+    none = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device="cuda")  # noqa: E731
+    q, bt, lens = none(0, 16, 128, dtype=torch.float16), none(0, 2), none(0)
+    out, lse = L.attn_decode_window(*b.cache, q, bt, lens, 5, want_lse=True)
+    assert out.shape == (0, 16, 128) and lse.shape == (0, 16)
+    assert L.attn_decode_weights(*b.cache, q, bt, lens, none(0, 64, dtype=torch.float32)).shape == (0, 16, 128)
+    start = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert L.attn_prefill_window(*b.cache, q, start, lens, lens, bt, 0, 5).shape == (0, 16, 128)
+    w = L.KvWeights(0, 2)
+    m = w.select(lens, 40)
+    L.kv_move(*b.cache, bt, m)
+    L.check_status()
+
+
+@pytest.mark.parametrize("op", ["window", "weights", "prefill", "move"])
+def test_pages_past_32_bit_offsets(op):
+    """A cache of 5 GB a side whose pages lie at its end: cells past 2^31 elements and bytes."""
+    Hkv, n = 8, 100
+    n_pages = (1 << 31) // (32 * Hkv * 128) + 8192  # 2^31 elements and 0.27 G more
+    b = Batch([n], 16, Hkv, seed=15)
+    big = [torch.empty(n_pages * 32, Hkv, 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+    pages = [n_pages - 1, n_pages - 17, 3, n_pages - 2]
+    bt = torch.tensor([pages], dtype=torch.int32, device="cuda")
+    for i, page in enumerate(pages):
+        src = int(b.bt_host[0, i]) * 32
+        for x, y in zip(big, b.cache):
+            x[page * 32:(page + 1) * 32] = y[src:src + 32]
+    start, pos0 = torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([n - 1], dtype=torch.int32, device="cuda")
+    if op == "move":
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        L.kv_move(*big, bt, L.KvMoves(i32([2]), i32([[97, 99]]), i32([[0, 40]]), 90))
+        L.check_status()
+        for x, y in zip(big, b.cache):
+            c = b.cells(0)
+            assert torch.equal(x[pages[0] * 32], y[int(c[97])]) and torch.equal(x[pages[1] * 32 + 8], y[int(c[99])])
+        return
+    if op == "window":
+        got, want = (L.attn_decode_window(*c, b.q, t, b.lens_t, 50, 3) for c, t in ((big, bt), (b.cache, b.bt)))
+    elif op == "weights":
+        accs = [torch.zeros(1, 128, device="cuda") for _ in range(2)]
+        got, want = (L.attn_decode_weights(*c, b.q, t, b.lens_t, a) for c, t, a in ((big, bt, accs[0]), (b.cache, b.bt, accs[1])))
+        assert torch.equal(*accs)
+    else:
+        got, want = (L.attn_prefill_window(*c, b.q, start, pos0, b.lens_t, t, 1, 50, 3)
+                     for c, t in ((big, bt), (b.cache, b.bt)))
+    L.check_status()
+    assert torch.equal(got, want)

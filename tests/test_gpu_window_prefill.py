@@ -73,6 +73,25 @@ def test_many_tiles_and_items(out_dtype):
     c.check(c.run(640, 50, out_dtype=out_dtype), 640, 50)
 
 
+def test_more_sequences_than_the_schedule_sorts():
+    """150 short sequences (some without queries or keys), taken in their own order."""
+    rng = np.random.default_rng(4)
+    seqs = []
+    for i in range(150):
+        t = int(rng.integers(0, 40))
+        seqs.append((int(rng.integers(0, 90)), t, 0)) if i % 29 == 5 else seqs.append((n := int(rng.integers(0, 90)), t, n + t))
+    for window, n_sink in ((33, 4), (500, 0)):
+        c = Chunks(seqs, 8, 2, seed=9)
+        c.check(c.run(window, n_sink, out_dtype=torch.bfloat16), window, n_sink)
+
+
+@pytest.mark.parametrize("T", [1, 16, 33, 64, 65, 300])
+def test_one_sequence(T):
+    for p0 in (0, 777):
+        c = Chunks([(p0, T, p0 + T)], 16, 8, seed=T)
+        c.check(c.run(100, 5), 100, 5)
+
+
 def test_rows_that_see_nothing_and_rows_of_no_sequence():
     """Keys end before some queries' windows begin: those rows are zeros; spare rows are left alone."""
     seqs = [(100, 100, 120), (500, 40, 100), (10, 30, 0)]
