@@ -80,7 +80,7 @@ constexpr int kSorted = 128;  // sequences that the schedule sorts (more are tak
 constexpr int kOffQ = 0;
 constexpr int kOffKv = 2 * kTile;
 constexpr int kOffBar = kOffKv + kStages * kTile;
-constexpr int kSmemBytes = kOffBar + 3072;
+constexpr int kSmemBytes = kOffBar + 3 * 1024;
 
 struct Barriers {
     uint64_t q_full;            // Q of both tiles landed (one phase per item)
@@ -100,7 +100,7 @@ struct Barriers {
     int first_pair[kSorted + 1];  // sorted schedule: pairs before each place of the order
     uint8_t order[kSorted];       // sequences, the most key tiles per pair first
 };
-static_assert(sizeof(Barriers) <= 3072, "barrier block over its reserved bytes");
+static_assert(sizeof(Barriers) <= 3 * 1024, "barrier block over its reserved bytes");
 static_assert(kSmemBytes <= 232448, "shared memory over the 227 KiB limit");
 
 // Bit i: key i of page pg is at a position below n.
