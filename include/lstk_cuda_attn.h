@@ -422,8 +422,14 @@ int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, co
  * queries are neither read nor computed, and block_tables entries of pages that no query sees are
  * not looked at. out is f32 or bf16 (out_dtype; each f32 result rounded once). Cells that no query of
  * the 256 rows computed together sees may hold anything; a non-finite K or V value that one of them
- * does see may reach the others. Other arguments, workspace and limits as lstk_cuda_attn_prefill; the _q8 form
+ * does see may reach the others. Few queries behind long contexts are split along the keys over the
+ * idle SMs, when the workspace holds lstk_cuda_attn_prefill_window_workspace_size bytes (for the current
+ * device, 256-byte aligned); one of lstk_cuda_attn_prefill_workspace_size bytes runs unsplit, with the same
+ * results up to f32 summation order. Other arguments and limits as lstk_cuda_attn_prefill; the _q8 form
  * as lstk_cuda_attn_prefill_q8 (same scratch), dequantising only the pages that some query sees. */
+size_t lstk_cuda_attn_prefill_window_workspace_size(int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                                                    int32_t max_q_len, int32_t max_blocks_per_seq, int64_t total_tokens,
+                                                    int32_t q_dtype, int32_t window, int32_t n_sink);
 int lstk_cuda_attn_prefill_window(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache,
                                   const void *q, int32_t q_dtype, int32_t n_seqs, int32_t n_head,
                                   const int32_t *q_seq_start, int32_t max_q_len, int64_t total_tokens,

@@ -27,5 +27,6 @@ from .bounded import (  # noqa: F401,E402
     attn_decode_window_q8,
     attn_prefill_window,
     attn_prefill_window_q8,
+    prefill_window_workspace_bytes,
 )
 from .evict import KvMoves, KvWeights, kv_move, kv_move_q8  # noqa: F401,E402

@@ -139,6 +139,8 @@ def lib():
     L.lstk_cuda_attn_prefill_workspace_size.restype = _SZ
     L.lstk_cuda_attn_prefill.argtypes = [_LP, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _I32, _F, _P,
                                          _P, _SZ, _P]
+    L.lstk_cuda_attn_prefill_window_workspace_size.argtypes = [_I32, _I32, _I32, _I32, _I32, _I32, _I64, _I32, _I32, _I32]
+    L.lstk_cuda_attn_prefill_window_workspace_size.restype = _SZ
     L.lstk_cuda_attn_prefill_window.argtypes = [_LP, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _I32, _I32,
                                                 _I32, _F, _P, _I32, _P, _SZ, _P]
     L.lstk_cuda_attn_prefill_window_q8.argtypes = [_LP, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P,

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, host, lib
-from .attn import HEAD_DIM
+from .attn import _DT, HEAD_DIM
 from .q8 import Q8Cache
 
 
@@ -81,13 +81,24 @@ def attn_decode_weights_q8(kq: Q8Cache, vq: Q8Cache, q, block_tables, seq_lens, 
     return (out, lse_out) if want_lse else out
 
 
+def prefill_window_workspace_bytes(q, n_head_kv, max_q_len, block_tables, window, n_sink=0):
+    """Bytes of workspace with which attn_prefill_window splits a call of these shapes along the keys where
+    that pays (on the current device)."""
+    total, Hq, _ = q.shape
+    return lib().lstk_cuda_attn_prefill_window_workspace_size(
+        block_tables.shape[0], Hq, n_head_kv, HEAD_DIM, int(max_q_len), block_tables.shape[1], total, _DT[q.dtype],
+        int(window), int(n_sink))
+
+
 def attn_prefill_window(k_cache, v_cache, q, q_seq_start, q_pos0, kv_lens, block_tables, max_q_len, window, n_sink=0,
                         scale=None, out=None, out_dtype=torch.float32, workspace=None, stream=None):
     """attn_prefill restricted to a sliding window and sinks: the query at position p sees its last
     `window` keys up to p (its own among them) and the first `n_sink`, all below kv_lens.
 
     Tiles that no query sees are neither read nor computed. out (or out_dtype) is f32 or bf16; a query
-    that sees no key gets zeros. Other arguments as attn_prefill."""
+    that sees no key gets zeros. workspace: uint8, None to allocate one that lets few queries behind long
+    contexts be split over the SMs (prefill_window_workspace_bytes); a smaller one, of at least
+    lstk_cuda_attn_prefill_workspace_size bytes, runs unsplit. Other arguments as attn_prefill."""
     rc, out = host().prefill(k_cache, None, v_cache, None, q, q_seq_start, q_pos0, kv_lens, block_tables, max_q_len,
                              window, n_sink, scale, out, out_dtype, workspace, None, stream)
     if rc:

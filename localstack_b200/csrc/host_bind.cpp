@@ -304,9 +304,14 @@ PyObject *prefill(PyObject *const *a) {
     if (!out.defined()) out = at::empty(q.sizes(), q.options().dtype(type));
     if (B == 0 || q.size(0) == 0) return result(LSTK_OK, out);
     const int32_t Hq = (int32_t) q.size(1), hkv = c.layout.n_head_kv;
-    const size_t need = lstk_cuda_attn_prefill_workspace_size((int32_t) B, Hq, hkv, (int32_t) kD, max_q, max_blocks,
-                                                              q.size(0), dtype_of(q));
-    if (bytes(ws) < need) ws = scratch(need, q);
+    // A workspace of the caller's that holds the f16 queries is used as it is (it may be too small to split
+    // the keys); otherwise one that allows the split.
+    if (!ws.defined() || bytes(ws) < lstk_cuda_attn_prefill_workspace_size((int32_t) B, Hq, hkv, (int32_t) kD, max_q,
+                                                                           max_blocks, q.size(0), dtype_of(q))) {
+        const size_t need = lstk_cuda_attn_prefill_window_workspace_size((int32_t) B, Hq, hkv, (int32_t) kD, max_q, max_blocks,
+                                                                         q.size(0), dtype_of(q), win, sink);
+        if (need) ws = scratch(need, q);
+    }
     const int32_t *start = static_cast<int32_t *>(ptr(i[0])), *pos0 = static_cast<int32_t *>(ptr(i[1]));
     const int32_t *lens = static_cast<int32_t *>(ptr(i[2])), *tables = static_cast<int32_t *>(ptr(i[3]));
     int rc;

@@ -39,7 +39,7 @@ struct DeviceInfo {
     size_t decode_q8_smem = 0;
     size_t decode_mode_smem[2][3] = {};  // per [q8_0][mode] (windowed, with accumulated weights)
     size_t prefill_smem = 0;
-    size_t prefill_window_smem[2] = {};  // per out_dtype (f32, bf16)
+    size_t prefill_window_smem[3] = {};  // f32 output, bf16 output, split along the keys
     size_t append_smem[8] = {};  // per kv_append instantiation (append_kernel)
     size_t gemm_smem = 0;
     size_t evict_smem[2] = {};  // per select_kernel instantiation (one CTA per row, a cluster)
@@ -938,6 +938,42 @@ static int check_prefill(const char *fn, const lstk_kv_layout *layout, const voi
     return LSTK_OK;
 }
 
+// Runs that the key tiles of a windowed prefill's items are cut into: enough to give every SM one, with at
+// least two key tiles each (a run's set-up and the join cost about as much as two tiles' chains, 2 us
+// each). 1 where the items alone occupy more than half of the SMs.
+static int prefill_window_splits(int n_sms, int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t max_q_len,
+                                 int32_t max_blocks, int32_t window, int32_t n_sink) {
+    const int tokens = 2 * (prefill::kBM / (n_head / n_head_kv));
+    const int64_t items = (int64_t) n_seqs * ((max_q_len + tokens - 1) / tokens) * n_head_kv;
+    const int64_t pages = std::min<int64_t>(max_blocks, ((int64_t) window + tokens + 62) / 32 + ((int64_t) n_sink + 31) / 32);
+    const int64_t tiles = (pages + 3) / 4;
+    if (items <= 0) return 1;
+    return (int) std::max<int64_t>(1, std::min<int64_t>({n_sms / items, tiles / 2, (int64_t) prefill_window::kMaxSplit}));
+}
+static size_t prefill_window_part_bytes(int splits, int32_t n_head, int64_t total_tokens) {
+    if (splits <= 1) return 0;
+    return align_up(sizeof(float) * (size_t) splits * total_tokens * n_head, 256) +
+           sizeof(float) * (size_t) splits * total_tokens * n_head * prefill::kD;
+}
+
+size_t lstk_cuda_attn_prefill_window_workspace_size(int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
+                                                    int32_t max_q_len, int32_t max_blocks_per_seq, int64_t total_tokens,
+                                                    int32_t q_dtype, int32_t window, int32_t n_sink) {
+    const size_t plain = lstk_cuda_attn_prefill_workspace_size(n_seqs, n_head, n_head_kv, head_dim, max_q_len,
+                                                               max_blocks_per_seq, total_tokens, q_dtype);
+    if (n_seqs <= 0 || n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv != 0 || n_head / n_head_kv > prefill::kBM ||
+        max_q_len <= 0 || max_blocks_per_seq <= 0 || total_tokens <= 0 || window < 1 || n_sink < 0)
+        return plain;
+    int dev = 0, n_sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        return plain;
+    }
+    const int splits = prefill_window_splits(n_sms, n_seqs, n_head, n_head_kv, max_q_len, max_blocks_per_seq, window, n_sink);
+    return align_up(plain, 256) + prefill_window_part_bytes(splits, n_head, total_tokens);
+}
+
 static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const void *v_cache, const void *q,
                         int32_t q_dtype, int32_t n_seqs, int32_t n_head, const int32_t *q_seq_start,
                         int32_t max_q_len, int64_t total_tokens, const int32_t *q_pos0, const int32_t *kv_lens,
@@ -995,11 +1031,27 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
     p.start_flag = t_start_flag;
     p.window = pw ? pw->window : 0;
     p.n_sink = pw ? pw->n_sink : 0;
+    p.n_split = 1;
+    p.max_q_len = max_q_len;
+    p.part_o = p.part_lse = nullptr;
+    if (pw) {
+        const size_t at = align_up(lstk_cuda_attn_prefill_workspace_size(n_seqs, n_head, hkv, layout->head_dim, max_q_len,
+                                                                         max_blocks_per_seq, total_tokens, q_dtype), 256);
+        const int splits = prefill_window_splits(dev->n_sms, n_seqs, n_head, hkv, max_q_len, max_blocks_per_seq, pw->window,
+                                                 pw->n_sink);
+        if (splits > 1 && workspace && aligned(workspace, 256) &&
+            workspace_bytes >= at + prefill_window_part_bytes(splits, n_head, total_tokens)) {
+            p.n_split = splits;
+            p.part_lse = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + at);
+            p.part_o = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + at +
+                                                 align_up(sizeof(float) * (size_t) splits * total_tokens * n_head, 256));
+        }
+    }
     const int64_t n_items = (int64_t) n_seqs * p.n_qt * hkv;
     if (n_items > (int64_t) INT32_MAX) return set_error(LSTK_ERR_CAPACITY, std::string(fn) + ": too many tiles");
     p.n_items = (int) n_items;
     // Persistent: one CTA per SM walks its share of the items (snake order over heaviest-first).
-    const int64_t grid = std::min<int64_t>(n_items, dev->n_sms);
+    const int64_t grid = std::min<int64_t>(n_items * p.n_split, dev->n_sms);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1007,8 +1059,10 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
     cfg.gridDim = dim3((unsigned) grid);
     if (pw) {
         const bool out16 = pw->out_dtype == LSTK_DTYPE_BF16;
-        const auto kernel = out16 ? prefill_window::prefill_window_kernel<true> : prefill_window::prefill_window_kernel<false>;
-        if ((rc = ensure_smem(&dev->prefill_window_smem[out16], kernel, prefill_window::kSmemBytes,
+        const auto kernel = p.n_split > 1 ? prefill_window::prefill_window_kernel<false, true>
+                            : out16       ? prefill_window::prefill_window_kernel<true, false>
+                                          : prefill_window::prefill_window_kernel<false, false>;
+        if ((rc = ensure_smem(&dev->prefill_window_smem[p.n_split > 1 ? 2 : out16], kernel, prefill_window::kSmemBytes,
                               "cudaFuncSetAttribute(prefill window)")))
             return rc;
         cfg.blockDim = dim3(prefill_window::kThreads);
@@ -1016,7 +1070,17 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
         cfg.stream = s;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        return launch_pdl_check(cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, p), "prefill_window_kernel");
+        rc = launch_pdl_check(cudaLaunchKernelEx(&cfg, kernel, qmap, kmap, vmap, p), "prefill_window_kernel");
+        if (rc || p.n_split == 1) return rc;
+        const int64_t warps = (int64_t) n_seqs * max_q_len * n_head;  // at most 148 items of 256 rows, so far below 2^31
+        cfg.gridDim = dim3((unsigned) ((warps + 7) / 8));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        return launch_pdl_check(cudaLaunchKernelEx(&cfg,
+                                                   out16 ? prefill_window::prefill_join_kernel<true>
+                                                         : prefill_window::prefill_join_kernel<false>,
+                                                   p),
+                                "prefill_join_kernel");
     }
     if ((rc = ensure_smem(&dev->prefill_smem, prefill::prefill_kernel, prefill::kSmemBytes,
                           "cudaFuncSetAttribute(prefill)")))

@@ -46,6 +46,8 @@
 //   warp 19     clears the V rows that no query of the item sees, in shared memory, before they are
 //               multiplied (a cell outside the sequence or the window may hold anything: 0 * inf is
 //               not 0), and passes the stage on.
+// Few items (a handful of queries behind long contexts): the items' key tiles are split over the idle SMs
+// and joined by log-sum-exp (prefill_join_kernel).
 // TMEM: S_0 [0,128), S_1 [128,256), O_0 [256,384), O_1 [384,512); P_t in S_t's columns [0,32) and
 // [64,96). Every wait is on a parity at most one phase from the arrivals, and bounded; a warp whose
 // wait ran out keeps taking part in its tile's named barriers until the item ends.
@@ -66,7 +68,13 @@ using prefill::kTile;
 
 struct Params : prefill::Params {  // n_qt counts pairs of query tiles
     int window, n_sink;
+    // Few items: every item's key tiles are cut into n_split runs, each an item of its own whose rows' results
+    // (normalised, f32) and log-sum-exps (log2 units) go to part_o / part_lse, row (split, token, head).
+    int n_split;
+    int max_q_len;
+    float *part_o, *part_lse;
 };
+constexpr int kMaxSplit = 32;
 
 constexpr int kStages = 5;
 constexpr int kSoftmaxWarps = 16;
@@ -121,6 +129,7 @@ struct Item {
     int b, kvh, tok0, q_begin, n_q, kv_len, pos0, n_keys, n_tiles;
     bool bad_rows;     // the sequence's query rows are not inside [0, total_tokens): no rows, reported
     bool second;       // the pair's second tile has rows
+    int split, tile0;  // this run of the item's key tiles: tile0 .. tile0 + n_tiles - 1
     int n_sink_pages, first_page, n_pages;  // pages: n_sink_pages from page 0, then those from first_page on
     int first;         // first key of the first query's window (at most n_keys)
     __device__ __forceinline__ int page(int v) const { return v < n_sink_pages ? v : v - n_sink_pages + first_page; }
@@ -148,6 +157,7 @@ __device__ __forceinline__ Item item_of(const Params &p, int b, int qt, int kvh)
     it.n_sink_pages = min((min(p.n_sink, it.first) + kPage - 1) / kPage, it.first_page);
     it.n_pages = it.n_sink_pages + end_page - it.first_page;
     it.n_tiles = (it.n_pages * kPage + kBN - 1) / kBN;
+    it.split = it.tile0 = 0;
     return it;
 }
 
@@ -157,6 +167,7 @@ __device__ __forceinline__ Item item_of(const Params &p, int b, int qt, int kvh)
 // (index), so the long items are dealt out evenly and the short ones fill the last round.
 // Eight chunks of 450 to 511 tokens behind contexts of up to 16 thousand keys (window 4096): a CTA's
 // longest share is 4 x 33 key tiles dealt in the sequences' own order, 3 x 33 and a short item sorted.
+template <bool kSplit>
 struct Schedule {
     const int *first_pair;  // shared memory; nullptr: unsorted
     const uint8_t *order;
@@ -167,6 +178,14 @@ struct Schedule {
         return idx < n_items ? (int) idx : -1;
     }
     __device__ __forceinline__ Item item(const Params &p, int x) const {
+        if constexpr (!kSplit) return whole(p, x);
+        Item it = whole(p, x / p.n_split);
+        it.split = x % p.n_split;
+        it.tile0 = it.n_tiles * it.split / p.n_split;
+        it.n_tiles = it.n_tiles * (it.split + 1) / p.n_split - it.tile0;
+        return it;
+    }
+    __device__ __forceinline__ Item whole(const Params &p, int x) const {
         const int kvh = x % p.n_head_kv, y = x / p.n_head_kv;
         if (first_pair == nullptr) return item_of(p, y % p.n_seqs, p.n_qt - 1 - y / p.n_seqs, kvh);
         int lo = 0, hi = p.n_seqs - 1;  // the last place with first_pair <= y
@@ -179,8 +198,9 @@ struct Schedule {
 };
 
 // Fills the schedule's shared memory (every thread of the block; cost: scratch of kSorted ints).
-__device__ __forceinline__ Schedule make_schedule(const Params &p, int *first_pair, uint8_t *order, int *cost, int *pairs) {
-    if (p.n_seqs == 1 || p.n_seqs > kSorted) return {nullptr, nullptr, p.n_items};
+template <bool kSplit>
+__device__ __forceinline__ Schedule<kSplit> make_schedule(const Params &p, int *first_pair, uint8_t *order, int *cost, int *pairs) {
+    if (p.n_seqs == 1 || p.n_seqs > kSorted) return {nullptr, nullptr, p.n_items * (kSplit ? p.n_split : 1)};
     const int b = threadIdx.x, tokens = 2 * (kBM / p.group);
     if (b < p.n_seqs) {
         const int q0 = p.q_seq_start[b], q1 = p.q_seq_start[b + 1];
@@ -202,7 +222,7 @@ __device__ __forceinline__ Schedule make_schedule(const Params &p, int *first_pa
         if (rank == p.n_seqs - 1) first_pair[p.n_seqs] = before + pairs[b];
     }
     __syncthreads();
-    return {first_pair, order, first_pair[p.n_seqs] * p.n_head_kv};
+    return {first_pair, order, first_pair[p.n_seqs] * p.n_head_kv * (kSplit ? p.n_split : 1)};
 }
 
 // 32 score columns of this thread's row - page v of the item's list - with the keys that the row's query
@@ -275,8 +295,9 @@ __device__ __forceinline__ float row_max(const float (&sc)[32]) {
 
 extern __shared__ __align__(1024) uint8_t dyn_smem[];
 
-// kOut16: out is bf16, each f32 result rounded once.
-template <bool kOut16>
+// kOut16: out is bf16, each f32 result rounded once. kSplit: items are runs of key tiles (Params::n_split),
+// whose results go to part_o and part_lse (kOut16 does not matter).
+template <bool kOut16, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                      const __grid_constant__ CUtensorMap kmap,
                                                                      const __grid_constant__ CUtensorMap vmap,
@@ -324,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
     pdl_wait();
     pdl_launch_dependents();
     const int G = p.group;
-    const Schedule sched = make_schedule(p, bars->first_pair, bars->order, reinterpret_cast<int *>(bars->row[0][0]),
+    const Schedule<kSplit> sched = make_schedule<kSplit>(p, bars->first_pair, bars->order, reinterpret_cast<int *>(bars->row[0][0]),
                                          reinterpret_cast<int *>(bars->row[0][1]));
 
     // Every role walks the same items. Barrier phases come from running counts: key tile g of this CTA
@@ -378,10 +399,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                 }
                 return cell;
             };
-            int cur = load_chunk(0);
-            int nxt = I.n_pages > 32 ? load_chunk(1) : (int) p.n_cells;
-            for (int j = 0; j < I.n_tiles; j++) {
-                if (j > 0 && (j & 7) == 0) {  // next 32 pages: 8 tiles
+            const int tile0 = kSplit ? I.tile0 : 0;
+            int cur = load_chunk(tile0 / 8);
+            int nxt = (tile0 / 8 + 1) * 32 < I.n_pages ? load_chunk(tile0 / 8 + 1) : (int) p.n_cells;
+            for (int j = tile0; j < tile0 + I.n_tiles; j++) {
+                if (j > tile0 && (j & 7) == 0) {  // next 32 pages: 8 tiles
                     cur = nxt;
                     nxt = (j / 8 + 1) * 32 < I.n_pages ? load_chunk(j / 8 + 1) : (int) p.n_cells;
                 }
@@ -539,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                 if (!ok) break;
                 bool cleared = false;
                 for (int q = 0; q < 4; q++) {
-                    const int v = 4 * j + q;  // pages past the list are zeros already
+                    const int v = 4 * ((kSplit ? I.tile0 : 0) + j) + q;  // pages past the list are zeros already
                     const uint32_t m = v < I.n_pages ? window_mask(I.page(v), I.first, I.n_keys, p.n_sink) : 0xffffffffu;
                     if (m == 0xffffffffu) continue;
                     cleared = true;
@@ -600,11 +622,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                 // within the registers of 20 warps.
                 float sc[32];
                 float m_half = -INFINITY;
+                const int v0 = 4 * ((kSplit ? I.tile0 : 0) + j) + 2 * hf;  // this warp's first page of the tile
                 if (ok) {
                     tc_fence_after();
-                    load_scores(sc, scol, I, 4 * j + 2 * hf, lo, hi, p.n_sink);
+                    load_scores(sc, scol, I, v0, lo, hi, p.n_sink);
                     m_half = row_max(sc);
-                    load_scores(sc, scol + 32, I, 4 * j + 2 * hf + 1, lo, hi, p.n_sink);
+                    load_scores(sc, scol + 32, I, v0 + 1, lo, hi, p.n_sink);
                     m_half = fmaxf(m_half, row_max(sc)) * p.scale_log2;
                 }
                 if (any_of_tile(m_half > m + prefill::kRescaleThreshold)) {
@@ -639,10 +662,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                     // P row r in quarters of 16 keys (8 packed columns, over the first 32 of this warp's own 64 score
                     // columns), each handed to the PV MMAs while the next one is computed.
                     uint32_t pk[16];
-                    load_scores(sc, scol + 32, I, 4 * j + 2 * hf + 1, lo, hi, p.n_sink);
+                    load_scores(sc, scol + 32, I, v0 + 1, lo, hi, p.n_sink);
                     eight_pairs<0>(pk, sc, scale2, neg_mu2, sum2);  // keys 32 .. 63 first: their columns are not P's
                     eight_pairs<1>(pk + 8, sc, scale2, neg_mu2, sum2);
-                    load_scores(sc, scol, I, 4 * j + 2 * hf, lo, hi, p.n_sink);
+                    load_scores(sc, scol, I, v0, lo, hi, p.n_sink);
                     tmem_st8(scol + 16, pk);
                     tmem_st8(scol + 24, pk + 8);
                     auto written = [&](int c) {
@@ -676,6 +699,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                 sync_tile();
                 const float sum = l + bars->row[t][hf ^ 1][r];
                 const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                const int64_t row = (int64_t) (I.q_begin + tq) * p.n_head + head;
+                const int64_t part = kSplit ? (int64_t) I.split * p.total_tokens * p.n_head + row : row;
+                if (kSplit && live && ok && hf == 0) p.part_lse[part] = sum > 0.f ? m + __log2f(sum) : -INFINITY;
                 tc_fence_after();
                 if (ok) {
 #pragma unroll
@@ -687,8 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                             // a row that saw no key is zero, whatever its O holds
 #pragma unroll
                             for (int i = 0; i < 32; i++) o[i] = sum > 0.f ? o[i] * inv : 0.f;
-                            const int64_t at = ((int64_t) (I.q_begin + tq) * p.n_head + head) * kD + 64 * hf + 32 * c;
-                            if constexpr (kOut16) {
+                            const int64_t at = part * kD + 64 * hf + 32 * c;
+                            if constexpr (kOut16 && !kSplit) {
                                 uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + at);
 #pragma unroll
                                 for (int ch = 0; ch < 4; ch++) {
@@ -701,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                                     dst[ch] = make_uint4(w[0], w[1], w[2], w[3]);
                                 }
                             } else {
-                                float4 *dst = reinterpret_cast<float4 *>(p.out + at);
+                                float4 *dst = reinterpret_cast<float4 *>((kSplit ? p.part_o : p.out) + at);
 #pragma unroll
                                 for (int ch = 0; ch < 8; ch++)
                                     dst[ch] = make_float4(o[4 * ch], o[4 * ch + 1], o[4 * ch + 2], o[4 * ch + 3]);
@@ -713,6 +739,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&bars->o_free[t]));
+            } else if (kSplit && live) {  // an empty run
+                if (hf == 0)
+                    p.part_lse[((int64_t) I.split * p.total_tokens + I.q_begin + tq) * p.n_head + head] = -INFINITY;
             } else if (live) {
                 // no visible keys: the row's output is zero
                 const int64_t at = ((int64_t) (I.q_begin + tq) * p.n_head + head) * kD + 64 * hf;
@@ -736,6 +765,42 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     if (warp == kWarpMma0) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Joins the runs of split items: a warp per row (token of a sequence, head), lane s the log-sum-exp of
+// run s, then each lane four dims of every run that saw a key.
+template <bool kOut16>
+__global__ void __launch_bounds__(256) prefill_join_kernel(const Params p) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t w = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t per_seq = (int64_t) p.max_q_len * p.n_head;
+    const int64_t b = w / per_seq;
+    if (b >= p.n_seqs) return;
+    const int tq = (int) ((w - b * per_seq) / p.n_head), head = (int) (w % p.n_head);
+    const int q0 = p.q_seq_start[b], q1 = p.q_seq_start[b + 1];
+    if (q0 < 0 || q1 < q0 || q1 > p.total_tokens || tq >= q1 - q0) return;  // no row of a sequence
+    const int64_t rows = (int64_t) p.total_tokens * p.n_head, row = (int64_t) (q0 + tq) * p.n_head + head;
+    const float l = lane < p.n_split ? p.part_lse[lane * rows + row] : -INFINITY;
+    const float M = warp_max_xor(l, 1);
+    const float wt = M == -INFINITY ? 0.f : fast_exp2(l - M);  // 0 for an empty run
+    const float den = warp_sum_xor(wt, 1);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.n_split; s++) {
+        const float ws = __shfl_sync(0xffffffffu, wt, s);
+        if (ws == 0.f) continue;  // its part_o was not written
+        const float4 v = reinterpret_cast<const float4 *>(p.part_o + (s * rows + row) * kD)[lane];
+        o.x += ws * v.x, o.y += ws * v.y, o.z += ws * v.z, o.w += ws * v.w;
+    }
+    const float inv = M == -INFINITY ? 0.f : 1.f / den;
+    o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if constexpr (kOut16) {
+        const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(o.x, o.y), __floats2bfloat162_rn(o.z, o.w)};
+        reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + row * kD)[lane] =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&h[0]), *reinterpret_cast<const uint32_t *>(&h[1]));
+    } else {
+        reinterpret_cast<float4 *>(p.out + row * kD)[lane] = o;
+    }
 }
 
 }  // namespace prefill_window

@@ -68,6 +68,12 @@ def test_window_refusals(q8):
     assert _window(q8=q8, B=5000) == CAP
     assert _prefill(q8=q8, qd=F32, wsb=100) == CAP and _prefill(q8=q8, qd=F32, ws=None) in (ARG, CAP)
     assert _prefill(q8=q8, lay=_layout(hkv=4), Hq=12) == UNSUP  # a group of 3 does not tile 128 rows
+    size = L.lib().lstk_cuda_attn_prefill_window_workspace_size
+    plain = L.lib().lstk_cuda_attn_prefill_workspace_size
+    for bad in ((-1, 16, 8, 128, 4, 4, 4, F32, 10, 2), (1, 0, 8, 128, 4, 4, 4, F32, 10, 2), (1, 16, 8, 128, 4, 4, 4, F32, 0, 2),
+                (1, 16, 8, 128, 4, 4, -4, F32, 10, 2)):
+        assert size(*bad) == plain(*bad[:8])  # no split for what the call refuses
+    assert size(1, 16, 8, 128, 4, 4, 4, F32, 10, 2) >= plain(1, 16, 8, 128, 4, 4, 4, F32)
     assert _prefill(q8=q8, pos0=None) == ARG and _prefill(q8=q8, total=-1) == ARG
     if q8:
         assert _prefill(q8=True, sc=None) == ARG and _prefill(q8=True, scb=10) == CAP and _prefill(q8=True, sc=P + 16) == ARG

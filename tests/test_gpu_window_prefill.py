@@ -92,6 +92,24 @@ def test_one_sequence(T):
         c.check(c.run(100, 5), 100, 5)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("seqs,Hq,Hkv", [([(4999, 1, 5000)], 8, 8), ([(4000, 3, 4003), (100, 2, 102), (0, 0, 9)], 8, 2),
+                                         ([(2900, 70, 2970)], 32, 4), ([(9, 1, 10)] * 5 + [(3000, 1, 3001)], 16, 8)])
+def test_few_queries_behind_long_contexts(seqs, Hq, Hkv, q8):
+    """Split along the keys (a workspace that allows it), and not (none): both within the bounds of the exact
+    result, rows of no sequence left alone."""
+    T = sum(t for _, t, _ in seqs)
+    for window, n_sink, dtype in ((5000, 0, torch.float32), (1999, 33, torch.bfloat16), (2**31 - 1, 4, torch.float32)):
+        c = Chunks(seqs, Hq, Hkv, seed=T, q8=q8, spare_rows=2)
+        need = L.prefill_window_workspace_bytes(c.b.q, Hkv, c.max_q, c.b.bt, window, n_sink)
+        assert need > 0
+        for ws in (torch.full((need,), 0xff, dtype=torch.uint8, device="cuda"), torch.empty(256, dtype=torch.uint8, device="cuda")):
+            out = torch.full((T + 2, Hq, 128), 7.0, dtype=dtype, device="cuda")
+            c.run(window, n_sink, out=out, workspace=ws)
+            c.check(out[:T], window, n_sink)
+            assert (out[T:] == 7).all()
+
+
 def test_rows_that_see_nothing_and_rows_of_no_sequence():
     """Keys end before some queries' windows begin: those rows are zeros; spare rows are left alone."""
     seqs = [(100, 100, 120), (500, 40, 100), (10, 30, 0)]
@@ -150,7 +168,8 @@ def test_graph_on_another_stream():
     c = Chunks([(0, 100, 100), (200, 30, 230)], 8, 2, seed=8, q_dtype=torch.float32)
     b = c.b
     out = torch.empty_like(b.q, dtype=torch.bfloat16)
-    ws = torch.empty(b.q.numel() * 2 + 256, dtype=torch.uint8, device="cuda")
+    ws = torch.empty(max(b.q.numel() * 2 + 256, L.prefill_window_workspace_bytes(b.q, 2, c.max_q, b.bt, 40, 3)),
+                     dtype=torch.uint8, device="cuda")
     c.run(40, 3, out=out, workspace=ws)
     g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
     with torch.cuda.graph(g, stream=side):
