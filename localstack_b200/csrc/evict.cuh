@@ -227,12 +227,21 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const SelectP
             __reduce_add_sync(0xffffffffu, mine.gt_high), __reduce_add_sync(0xffffffffu, mine.eq_high)};
     if (lane == 0) warp_counts[warp] = mine;
     __syncthreads();
-    Counts before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
+    // Every warp: lane w the counts of warp w, scanned; `before` of this warp, `all` of the CTA.
+    Counts scan = lane < kSelectWarps ? warp_counts[lane] : Counts{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < kSelectWarps; w++) {
-        if (w == warp) before = all;
-        all.add(warp_counts[w]);
+    for (int off = 1; off < kSelectWarps; off <<= 1) {
+        const Counts o = {__shfl_up_sync(0xffffffffu, scan.gt_low, off), __shfl_up_sync(0xffffffffu, scan.eq_low, off),
+                          __shfl_up_sync(0xffffffffu, scan.gt_high, off), __shfl_up_sync(0xffffffffu, scan.eq_high, off)};
+        if (lane >= off) scan.add(o);
     }
+    auto of_lane = [&](int l) {
+        return Counts{__shfl_sync(0xffffffffu, scan.gt_low, l), __shfl_sync(0xffffffffu, scan.eq_low, l),
+                      __shfl_sync(0xffffffffu, scan.gt_high, l), __shfl_sync(0xffffffffu, scan.eq_high, l)};
+    };
+    const Counts all = of_lane(kSelectWarps - 1), upto = of_lane(warp);
+    const Counts before = {upto.gt_low - mine.gt_low, upto.eq_low - mine.eq_low, upto.gt_high - mine.gt_high,
+                           upto.eq_high - mine.eq_high};
     if (kMulti) {
         if (tid == 0) cta_counts = all;
         cluster.sync();
