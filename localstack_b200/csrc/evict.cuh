@@ -117,16 +117,16 @@ struct __align__(16) Counts {
 // warp with a contiguous stretch of its CTA's. The budget-th largest key is found 8 bits at a time:
 // shared-memory histograms of the keys that match the bits found so far (one array per step, so that no
 // CTA clears what another still reads), copied once from the cluster's other CTAs (1 KiB each, through
-// distributed shared memory), and then every warp sums and scans the 256 bins for itself, without a
-// further barrier. The ranks of equal keys, of holes and of movers come from ballots, the warps' counts,
-// and one exchange of the CTAs' counts (an equal key's rank decides whether it stays, and equal keys in
-// low indexes come before those in high ones, so the counts of kept keys follow from Counts alone).
+// distributed shared memory), summed and scanned by one warp. The ranks of equal keys, of holes and of
+// movers come from ballots, the warps' counts, and one exchange of the CTAs' counts (an equal key's rank
+// decides whether it stays, and equal keys in low indexes come before those in high ones, so the counts
+// of kept keys follow from Counts alone).
 // The weights and positions are read once; the rest is latency: the launch, two round trips to memory,
 // and the barriers of four steps and one exchange. Measured with the moves, as a call of both: one row of
-// 544 keys 11 us, 64 rows of 4 k 16 us, 16 rows of up to 32 k cut to 8 k 62 us (moves 38). Three steps of
-// 11 bits took longer (16 rows: selection 26 us against 19): the cluster's 8 KiB histograms cost more to
-// read than the fourth step saves; so did aggregating equal keys before the atomics (26 against 19). 1024
-// threads against 512: 64 rows 16.0 against 18.0 us, 16 rows 61.4 against 66.7, one row the same.
+// 544 keys 11 us, 64 rows of 4 k 13 us, 16 rows of up to 32 k cut to 8 k 56 us (moves 36). Steps that paid
+// there: 8 bits at a time instead of 11 (the cluster's 8 KiB histograms cost more to read than a fourth
+// step), plain atomics instead of aggregating equal keys first, 1024 threads instead of 512 (18.0 -> 16.0
+// and 66.7 -> 61.4 us), one warp scanning instead of all 32 (14.4 -> 12.9 and 60.5 -> 56.3 us).
 // The loops are kept rolled: code that runs once per launch costs its instruction fetches.
 template <bool kMulti>
 __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const SelectParams p) {
@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const SelectP
     __shared__ __align__(16) int hist[4][kBins];  // read as int4
     __shared__ __align__(16) int parts[kMulti ? kMaxCluster : 1][kBins];
     __shared__ Counts warp_counts[kSelectWarps], cta_counts;
+    __shared__ uint32_t found_s[2];  // the bits found so far, and the keys still to be taken
     cg::cluster_group cluster = cg::this_cluster();
     const int C = kMulti ? (int) cluster.num_blocks() : 1, rank = kMulti ? (int) cluster.block_rank() : 0;
     const int b = blockIdx.x / C;
@@ -186,33 +187,40 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const SelectP
             if (r < C) reinterpret_cast<int4 *>(parts[r])[q] = reinterpret_cast<const int4 *>(cluster.map_shared_rank(&hist[d][0], r))[q];
         }
         __syncthreads();
-        // lane l: bins 255 - 8 l down to 248 - 8 l
-        int c[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0;
+        if (warp == 0) {  // one warp: 32 that scan for themselves take 1300 cycles of issue slots, this 500
+            // lane l: bins 255 - 8 l down to 248 - 8 l
+            int c[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0;
 #pragma unroll
-        for (int r = 0; r < (kMulti ? kMaxCluster : 1); r++) {
-            if (kMulti && r >= C) break;
-            const int4 *h = reinterpret_cast<const int4 *>(kMulti ? parts[r] : hist[d]) + 2 * (31 - lane);
-            const int4 u = h[0], v = h[1];
-            c[0] += v.w, c[1] += v.z, c[2] += v.y, c[3] += v.x, c[4] += u.w, c[5] += u.z, c[6] += u.y, c[7] += u.x;
+            for (int r = 0; r < (kMulti ? kMaxCluster : 1); r++) {
+                if (kMulti && r >= C) break;
+                const int4 *h = reinterpret_cast<const int4 *>(kMulti ? parts[r] : hist[d]) + 2 * (31 - lane);
+                const int4 u = h[0], v = h[1];
+                c[0] += v.w, c[1] += v.z, c[2] += v.y, c[3] += v.x, c[4] += u.w, c[5] += u.z, c[6] += u.y, c[7] += u.x;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum += c[e];
+            int above = sum;  // of the bins over this lane's
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, above, off);
+                if (lane >= off) above += y;
+            }
+            above -= sum;
+            const uint32_t has = __ballot_sync(0xffffffffu, above < need && need <= above + sum);  // exactly one lane
+            int digit = 255 - 8 * lane;
+#pragma unroll
+            for (int e = 0; e < 7; e++) {
+                if (need > above + c[e] && digit == 255 - 8 * lane - e) above += c[e], digit--;
+            }
+            const int from = __ffs((int) has) - 1;
+            if (lane == from) {
+                found_s[0] = (prefix << 8) | (uint32_t) digit;
+                found_s[1] = (uint32_t) (need - above);
+            }
         }
-#pragma unroll
-        for (int e = 0; e < 8; e++) sum += c[e];
-        int above = sum;  // of the bins over this lane's
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, above, off);
-            if (lane >= off) above += y;
-        }
-        above -= sum;
-        const uint32_t has = __ballot_sync(0xffffffffu, above < need && need <= above + sum);  // exactly one lane
-        int digit = 255 - 8 * lane;
-#pragma unroll
-        for (int e = 0; e < 7; e++) {
-            if (need > above + c[e] && digit == 255 - 8 * lane - e) above += c[e], digit--;
-        }
-        const int from = __ffs((int) has) - 1;
-        prefix = (prefix << 8) | (uint32_t) __shfl_sync(0xffffffffu, digit, from);
-        need -= __shfl_sync(0xffffffffu, above, from);
+        __syncthreads();
+        prefix = found_s[0];
+        need = (int) found_s[1];
     }
     // Kept: key > prefix, and the first `need` keys equal to it.
     const int edge = p.budget - first;  // indexes below it are low
