@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -140,9 +141,13 @@ void same_device(const at::Tensor &a, const at::Tensor &b) {
 void *ptr(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 size_t bytes(const at::Tensor &t) { return t.defined() ? (size_t) t.nbytes() : 0; }
 
-at::Tensor scratch(size_t n, const at::Tensor &like) {
-    return at::empty({(int64_t) n}, like.options().dtype(at::kByte));
+// An uninitialised tensor on the device of `like`, from torch's allocator (without the dispatcher's
+// way there, which costs as much again).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like) {
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
+
+at::Tensor scratch(size_t n, const at::Tensor &like) { return fresh({(int64_t) n}, at::kByte, like); }
 
 PyObject *wrap(const at::Tensor &t) {
     if (t.defined()) return THPVariable_Wrap(t);
@@ -193,8 +198,8 @@ struct Decode {
         for (const at::Tensor *t : Tensors{&c.kd, &c.v, &c.vd, &q, &tables, &lens, &out, &lse}) same_device(c.k, *t);
     }
     void allocate() {
-        if (!out.defined()) out = at::empty(q.sizes(), q.options().dtype(type));
-        if (want_lse && !lse.defined()) lse = at::empty({B, Hq}, q.options().dtype(at::kFloat));
+        if (!out.defined()) out = fresh(q.sizes(), type, q);
+        if (want_lse && !lse.defined()) lse = fresh({B, Hq}, at::kFloat, q);
     }
 };
 
@@ -301,7 +306,7 @@ PyObject *prefill(PyObject *const *a) {
     else type = out_type(a[14]);
     for (const at::Tensor *t : Tensors{&c.kd, &c.v, &c.vd, &q, &i[0], &i[1], &i[2], &i[3], &out, &ws, &sc}) same_device(c.k, *t);
     OnStream s(a[17], c.k.device());
-    if (!out.defined()) out = at::empty(q.sizes(), q.options().dtype(type));
+    if (!out.defined()) out = fresh(q.sizes(), type, q);
     if (B == 0 || q.size(0) == 0) return result(LSTK_OK, out);
     const int32_t Hq = (int32_t) q.size(1), hkv = c.layout.n_head_kv;
     // A workspace of the caller's that holds the f16 queries is used as it is (it may be too small to split
@@ -356,9 +361,9 @@ PyObject *select(PyObject *const *a) {
     for (const at::Tensor *t : Tensors{&lens, &n, &src, &dst}) same_device(acc, *t);
     OnStream s(a[11], acc.device());
     if (!n.defined()) {
-        n = at::empty({rows}, lens.options());
-        src = at::empty({rows, most}, lens.options());
-        dst = at::empty({rows, most}, lens.options());
+        n = fresh({rows}, at::kInt, acc);
+        src = fresh({rows, most}, at::kInt, acc);
+        dst = fresh({rows, most}, at::kInt, acc);
     }
     if (rows == 0) return result(LSTK_OK, n, src, dst);
     const lstk_kv_weights w = {static_cast<float *>(ptr(acc)), static_cast<int32_t *>(ptr(pos)),
