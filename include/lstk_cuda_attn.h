@@ -170,7 +170,8 @@ int lstk_cuda_attn_decode_static(const lstk_kv_layout *layout, const void *k_cac
  * pages that hold visible keys are read: entries of block_tables between the sinks' last page and
  * the window's first are not looked at, so the host may have reused those pages. Arguments, results,
  * workspace and limits as lstk_cuda_attn_decode, except: out is f32 or bf16 (out_dtype; bf16, the input
- * type of lstk_cuda_proj, rounds each f32 result once), and lse_out covers the visible keys.
+ * type of lstk_cuda_proj, rounds each f32 result once), and lse_out covers the visible keys. A NaN among a
+ * row's visible scores makes its out and lse NaN. out does not overlap q.
  * max_seq_len bounds seq_lens as there (it sizes the launch only). The _q8 form reads a q8_0 cache
  * with lstk_cuda_attn_decode_q8's semantics, the query's block scale taken as amax * (1 / 127) in f32
  * (a product: its last bit may differ from the quotient's there). */
@@ -196,7 +197,8 @@ int lstk_cuda_attn_decode_window_q8(const lstk_kv_layout *layout, const int8_t *
  * acc hold at least max_seq_len keys (0 = max_blocks * block_size), and so does the workspace
  * (lstk_cuda_attn_decode_weights_workspace_size, which includes the scores of the step: n_head * 4
  * bytes per key); a sequence longer than max_seq_len reports LSTK_ERR_DEVICE_INDEX and attends to its
- * first max_seq_len keys only. A key whose page id is out of range has no weight. The _q8 form as
+ * first max_seq_len keys only. A key whose page id is out of range has no weight. A query row with a NaN
+ * among its scores makes its out and lse, and the sequence's weights, NaN. The _q8 form as
  * lstk_cuda_attn_decode_window_q8. */
 size_t lstk_cuda_attn_decode_weights_workspace_size(int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
                                                     int32_t max_seq_len);
@@ -422,7 +424,8 @@ int lstk_cuda_attn_prefill(const lstk_kv_layout *layout, const void *k_cache, co
  * queries are neither read nor computed, and block_tables entries of pages that no query sees are
  * not looked at. out is f32 or bf16 (out_dtype; each f32 result rounded once). Cells that no query of
  * the 256 rows computed together sees may hold anything; a non-finite K or V value that one of them
- * does see may reach the others. Few queries behind long contexts are split along the keys over the
+ * does see may reach the others (a NaN key makes the rows that see it NaN). scale is positive and finite.
+ * out does not overlap q. Few queries behind long contexts are split along the keys over the
  * idle SMs, when the workspace holds lstk_cuda_attn_prefill_window_workspace_size bytes (for the current
  * device, 256-byte aligned); one of lstk_cuda_attn_prefill_workspace_size bytes runs unsplit, with the same
  * results up to f32 summation order. Other arguments and limits as lstk_cuda_attn_prefill; the _q8 form

@@ -918,7 +918,10 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
                         const int n = 2 * t + h;
                         if (n >= p.group) continue;
                         const float inv = l[h] > 0.f ? 1.f / l[h] : 0.f;
-                        const float lse2 = l[h] > 0.f ? st.m[h] + __log2f(l[h]) : -INFINITY;
+                        float lse2 = l[h] > 0.f ? st.m[h] + __log2f(l[h]) : -INFINITY;
+                        // A row with a NaN among its visible scores is NaN: o is, and a piece's +inf makes the
+                        // combine's weights NaN. (kPlain leaves such a piece out.)
+                        if (kMode != kPlain && l[h] != l[h]) lse2 = whole ? NAN : INFINITY;
                         float *dst;
                         if (kMode != kPlain && whole && p.out_bf16) {
                             const int64_t row = (int64_t) cur.b * p.n_head + (int64_t) kvh * p.group + n;
@@ -1321,8 +1324,8 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
                 if (tid < nd) o += acc_s[k][tid] * f;
             }
         }
-        o = total > 0.f ? o / total : 0.f;
-        row_lse = total > 0.f ? (M + __log2f(total)) * 0.69314718055994531f : -INFINITY;
+        o = total != 0.f ? o / total : 0.f;
+        row_lse = total != 0.f ? (M + __log2f(total)) * 0.69314718055994531f : -INFINITY;
     }
     finish_row<kExchange, kTyped>(p, out_row, d0, nd, o, row_lse, xs);
     advance_epoch<kExchange>(p, xs);
@@ -1417,9 +1420,9 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_rows_kernel
     }
     // Divided as decode_combine_kernel divides: a row of up to 8 pieces then gets the same bits
     // from both kernels (the same weights, summed in piece order).
-    store(den > 0.f ? make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den) : make_float4(0.f, 0.f, 0.f, 0.f));
+    store(den != 0.f ? make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den) : make_float4(0.f, 0.f, 0.f, 0.f));
     if (lane == 0 && p.lse_out != nullptr)
-        p.lse_out[out_row] = den > 0.f ? (m + __log2f(den)) * 0.69314718055994531f : -INFINITY;
+        p.lse_out[out_row] = den != 0.f ? (m + __log2f(den)) * 0.69314718055994531f : -INFINITY;
 }
 
 // kWeights, after the combine: acc[b][i] += sum over the query rows r of 2^(score[r][i] - lse2[r]), the

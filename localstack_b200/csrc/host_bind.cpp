@@ -192,7 +192,9 @@ struct Decode {
         if (lse.defined())
             require(lse.scalar_type() == at::kFloat && lse.dim() == 2 && lse.size(0) == B && lse.size(1) == Hq && lse.is_contiguous(),
                     "lse_out must be a contiguous f32 [B][Hq] tensor");
-        want_lse = PyObject_IsTrue(want) == 1;
+        const int truth = PyObject_IsTrue(want);
+        if (truth < 0) throw python_error();
+        want_lse = truth == 1;
     }
     void check_devices(const Cache &c) const {
         for (const at::Tensor *t : Tensors{&c.kd, &c.v, &c.vd, &q, &tables, &lens, &out, &lse}) same_device(c.k, *t);

@@ -902,13 +902,15 @@ struct PrefillWindow {
     int32_t window, n_sink, out_dtype;
 };
 
-static int check_prefill_window(const PrefillWindow *pw, int32_t max_blocks_per_seq) {
+static int check_prefill_window(const PrefillWindow *pw, int32_t max_blocks_per_seq, float scale) {
     if (pw->out_dtype != LSTK_DTYPE_F32 && pw->out_dtype != LSTK_DTYPE_BF16)
         return set_error(LSTK_ERR_UNSUPPORTED, std::string(pw->fn) + ": out_dtype must be f32 or bf16");
     if (pw->window < 1 || pw->n_sink < 0)
         return set_error(LSTK_ERR_INVALID_ARG, std::string(pw->fn) + ": window must be at least 1 and n_sink at least 0");
     if (max_blocks_per_seq > INT32_MAX / 32)
         return set_error(LSTK_ERR_INVALID_ARG, std::string(pw->fn) + ": max_blocks_per_seq out of range");
+    if (!(scale > 0.f && scale < INFINITY))  // the row maxima are taken before it is multiplied in
+        return set_error(LSTK_ERR_INVALID_ARG, std::string(pw->fn) + ": scale must be positive and finite");
     return LSTK_OK;
 }
 
@@ -982,7 +984,7 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
     const char *fn = pw ? pw->fn : "lstk_cuda_attn_prefill";
     int rc = check_layout(layout, fn);
     if (rc) return rc;
-    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq))) return rc;
+    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq, scale))) return rc;
     if ((rc = check_prefill(fn, layout, k_cache, v_cache, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len,
                             total_tokens, q_pos0, kv_lens, block_tables, max_blocks_per_seq, out, workspace,
                             workspace_bytes)))
@@ -1140,7 +1142,7 @@ static int prefill_q8_impl(const lstk_kv_layout *layout, const int8_t *k_qs, con
     const char *fn = pw ? pw->fn : "lstk_cuda_attn_prefill_q8";
     int rc = check_layout(layout, fn);
     if (rc) return rc;
-    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq))) return rc;
+    if (pw && (rc = check_prefill_window(pw, max_blocks_per_seq, scale))) return rc;
     if (pw && (rc = check_prefill(fn, layout, k_qs, v_qs, q, q_dtype, n_seqs, n_head, q_seq_start, max_q_len,
                                   total_tokens, q_pos0, kv_lens, block_tables, max_blocks_per_seq, out, workspace,
                                   workspace_bytes)))

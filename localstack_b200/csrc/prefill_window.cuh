@@ -698,10 +698,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                 bars->row[t][hf][r] = l;
                 sync_tile();
                 const float sum = l + bars->row[t][hf ^ 1][r];
-                const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                const bool none = sum == 0.f;  // the row saw no key; a sum of NaN makes the row NaN
+                const float inv = 1.f / sum;
                 const int64_t row = (int64_t) (I.q_begin + tq) * p.n_head + head;
                 const int64_t part = kSplit ? (int64_t) I.split * p.total_tokens * p.n_head + row : row;
-                if (kSplit && live && ok && hf == 0) p.part_lse[part] = sum > 0.f ? m + __log2f(sum) : -INFINITY;
+                if (kSplit && live && ok && hf == 0) p.part_lse[part] = none ? -INFINITY : sum != sum ? INFINITY : m + __log2f(sum);
                 tc_fence_after();
                 if (ok) {
 #pragma unroll
@@ -712,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
                         if (live) {
                             // a row that saw no key is zero, whatever its O holds
 #pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] = sum > 0.f ? o[i] * inv : 0.f;
+                            for (int i = 0; i < 32; i++) o[i] = none ? 0.f : o[i] * inv;
                             const int64_t at = part * kD + 64 * hf + 32 * c;
                             if constexpr (kOut16 && !kSplit) {
                                 uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + at);
@@ -783,7 +784,7 @@ __global__ void __launch_bounds__(256) prefill_join_kernel(const Params p) {
     const int64_t rows = (int64_t) p.total_tokens * p.n_head, row = (int64_t) (q0 + tq) * p.n_head + head;
     const float l = lane < p.n_split ? p.part_lse[lane * rows + row] : -INFINITY;
     const float M = warp_max_xor(l, 1);
-    const float wt = M == -INFINITY ? 0.f : fast_exp2(l - M);  // 0 for an empty run
+    const float wt = M == -INFINITY ? 0.f : fast_exp2(l - M);  // 0 for an empty run, NaN for a run of NaN (+inf)
     const float den = warp_sum_xor(wt, 1);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s = 0; s < p.n_split; s++) {

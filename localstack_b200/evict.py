@@ -90,8 +90,11 @@ class KvWeights:
     def finish(self, pages, moves, stream=None):
         """Ends an eviction: acc and pos follow the moves, the rows of `pages` (a DevicePages) are
         truncated to the budget and their blocks freed. Call it once, after every layer's kv_move."""
-        if moves.src.shape[0] != self.n_rows:
+        if moves.n.shape != (self.n_rows,) or moves.src.shape[0] != self.n_rows or moves.dst.shape != moves.src.shape:
             raise ValueError("moves and weights must have the same rows")
+        if any(t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.device
+               for t in (moves.n, moves.src, moves.dst)):
+            raise ValueError("moves must be contiguous int32 tensors on the weights' device")
         check(lib().lstk_cuda_kv_evict_finish(ctypes.byref(pages.state), ctypes.byref(self.state), moves.budget,
                                               _p(moves.n), _p(moves.src), _p(moves.dst), moves.src.shape[1],
                                               _stream(stream, self.device)))

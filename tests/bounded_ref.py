@@ -23,6 +23,8 @@ row's maximum) to f16 - ln 2 * 2^-11 * |x| of the probability - and takes ex2.ap
 (relative 2^-9.9); the row sum adds the same rounded probabilities, so with d_i the sum of these
 
     |out - exact| <= sum_i p_i d_i (|v_i| + |out|) + 2^-25 sum_i (|v_i| + |out|)
+
+The windowed prefill takes its exponentials of f32 scores and in f32, which these bounds cover.
 """
 from __future__ import annotations
 

@@ -36,9 +36,9 @@ def _weights(q8=False, lay=None, bad="", q=P, qd=F16, B=1, Hq=16, bt=P, mb=4, le
 
 
 def _prefill(q8=False, lay=None, bad="", q=P, qd=F16, B=1, Hq=16, start=P, mq=4, total=4, pos0=P, lens=P, bt=P, mb=4,
-             window=10, sink=2, out=P, od=BF16, ws=P, wsb=BIG, sc=P, scb=BIG):
+             window=10, sink=2, out=P, od=BF16, ws=P, wsb=BIG, sc=P, scb=BIG, scale=0.1):
     fn = L.lib().lstk_cuda_attn_prefill_window_q8 if q8 else L.lib().lstk_cuda_attn_prefill_window
-    return fn(lay or _layout(), *_caches(q8, bad), q, qd, B, Hq, start, mq, total, pos0, lens, bt, mb, window, sink, 0.1,
+    return fn(lay or _layout(), *_caches(q8, bad), q, qd, B, Hq, start, mq, total, pos0, lens, bt, mb, window, sink, scale,
               out, od, ws, wsb, *((sc, scb) if q8 else ()), None)
 
 
@@ -74,6 +74,8 @@ def test_window_refusals(q8):
                 (1, 16, 8, 128, 4, 4, -4, F32, 10, 2)):
         assert size(*bad) == plain(*bad[:8])  # no split for what the call refuses
     assert size(1, 16, 8, 128, 4, 4, 4, F32, 10, 2) >= plain(1, 16, 8, 128, 4, 4, 4, F32)
+    for scale in (0.0, -0.1, float("nan"), float("inf")):
+        assert _prefill(q8=q8, scale=scale) == ARG and "scale" in _lib.last_error()
     assert _prefill(q8=q8, pos0=None) == ARG and _prefill(q8=q8, total=-1) == ARG
     if q8:
         assert _prefill(q8=True, sc=None) == ARG and _prefill(q8=True, scb=10) == CAP and _prefill(q8=True, sc=P + 16) == ARG
@@ -127,6 +129,15 @@ def test_eviction_refusals():
     assert fin(s=st(bs=16)) == UNSUP and fin(s=st(slots=3)) == ARG and fin(s=st(mb=5)) == ARG and fin(w=_state(pos=0)) == ARG
     assert fin(budget=0) == ARG and fin(cap=10) == ARG and fin(n=None) == ARG and fin(a=None) == ARG
     assert fin(s=st(mb=1 << 27)) == ARG
+
+
+def test_finish_checks_its_moves():
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    w = L.KvWeights(2, 4, device="cpu")
+    for moves in (L.KvMoves(i32(3), i32(3, 64), i32(3, 64), 64), L.KvMoves(i32(2), i32(2, 64), i32(2, 63), 64),
+                  L.KvMoves(i32(2).long(), i32(2, 64), i32(2, 64), 64), L.KvMoves(i32(2), i32(64, 2).t(), i32(2, 64), 64)):
+        with pytest.raises(ValueError):
+            w.finish(None, moves)
 
 
 def test_python_checks():

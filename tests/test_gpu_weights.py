@@ -163,3 +163,20 @@ def test_graph_on_another_stream():
         torch.cuda.synchronize()
         L.check_status()
         _check(b, out, lse, acc, torch.zeros_like(acc), steps=2)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("lens", [[20, 300], [600, 300], [5000, 300], list(range(20, 900, 40))])
+def test_a_nan_key_makes_its_rows_nan(lens, q8):
+    b = Batch(lens, 16, 4, seed=1, q8=q8)
+    for i in range(len(lens) - 1):
+        (b.cache[0].d if q8 else b.cache[0])[b.cells(i)[lens[i] - 5], 2] = float("nan")
+    acc = _acc(b)
+    before = acc.clone()
+    out, lse = _run(b, acc)
+    group = slice(8, 12)
+    assert out[:-1, group].isnan().all() and lse[:-1, group].isnan().all()
+    for i, n in enumerate(lens[:-1]):
+        assert acc[i, :n].isnan().all() and torch.equal(acc[i, n:], before[i, n:])
+    out[:-1, group] = 0
+    assert not out.isnan().any() and not acc[-1].isnan().any()

@@ -251,3 +251,31 @@ def test_pages_past_32_bit_offsets(op):
                      for c, t in ((big, bt), (b.cache, b.bt)))
     L.check_status()
     assert torch.equal(got, want)
+
+
+def _poison_keys(b, at, head):
+    """A NaN in KV head `head` of the key at(n) of every sequence but the last."""
+    for i in range(len(b.lens) - 1):
+        cell = b.cells(i)[at(b.lens[i])]
+        (b.cache[0].d if b.q8 else b.cache[0])[cell, head] = float("nan")
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens", [[20, 300], [600, 300], [5000, 300], list(range(20, 900, 40))])
+def test_a_nan_key_makes_the_rows_that_see_it_nan(lens, out_dtype, q8):
+    """Whether one CTA has the whole row or pieces of it are merged; other heads and sequences are not touched."""
+    b = Batch(lens, 16, 4, seed=1, q8=q8)
+    _poison_keys(b, lambda n: n - 5, 2)
+    out, lse = _run(b, 100000, 4, out_dtype=out_dtype)
+    group = slice(8, 12)
+    assert out[:-1, group].isnan().all() and lse[:-1, group].isnan().all()
+    out[:-1, group] = 0
+    lse[:-1, group] = 0
+    assert not out.isnan().any() and not lse.isnan().any()
+    out, lse = _run(b, 3, 4, out_dtype=out_dtype)  # out of the window
+    _check(b, out, lse, 3, 4)
+    b.q.fill_(float("nan"))
+    if not q8:
+        out, lse = _run(b, 100000, 4, out_dtype=out_dtype)
+        assert out.isnan().all() and lse.isnan().all()

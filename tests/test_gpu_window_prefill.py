@@ -185,3 +185,21 @@ def test_graph_on_another_stream():
     L.check_status()
     b.lens = [100, 180]
     c.check(out, 40, 3)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("seqs,window", [([(100, 140, 240)], 60), ([(0, 300, 300), (30, 90, 120)], 60),
+                                         ([(4990, 10, 5000)], 100000), ([(4970, 30, 5000), (100, 40, 140)], 4000)])
+def test_a_nan_key_makes_the_rows_that_see_it_nan(seqs, window, out_dtype, q8):
+    c = Chunks(seqs, 16, 4, seed=2, q8=q8)
+    b = c.b
+    at = [max(n - 120, 3) for _, _, n in seqs]
+    for i in range(len(seqs)):
+        (b.cache[0].d if q8 else b.cache[0])[b.cells(i)[at[i]], 2] = float("nan")
+    out = c.run(window, 2, out_dtype=out_dtype)
+    for i, (p0, t, n) in enumerate(seqs):
+        sees = torch.from_numpy(window_mask(p0 + np.arange(t), n, window, 2)[:, at[i]]).cuda()
+        o = out[c.starts[i]:c.starts[i + 1]]
+        assert torch.equal(o.isnan().all(-1), sees[:, None] & (torch.arange(16, device="cuda") // 4 == 2))
+        assert torch.equal(o.isnan().any(-1), o.isnan().all(-1))
