@@ -116,10 +116,12 @@ __device__ __forceinline__ uint32_t below(int n, int pg) {
     const int r = n - pg * kPage;
     return r <= 0 ? 0u : r >= kPage ? 0xffffffffu : (1u << r) - 1u;
 }
-// First key of the window of the query at position pos (a window of up to 2^31 - 1 keys).
-__device__ __forceinline__ int window_first(int pos, int window) {
-    return (int) max((int64_t) 0, (int64_t) pos + 1 - window);
+// First key of the window of the query at position pos, and one past its last key. Positions may pass 32
+// bits (a first position of up to 2^31 - 1, keys only below it).
+__device__ __forceinline__ int window_first(int64_t pos, int window) {
+    return (int) min(max((int64_t) 0, pos + 1 - window), (int64_t) INT32_MAX);
 }
+__device__ __forceinline__ int keys_end(int64_t pos, int kv_len) { return (int) max(min(pos + 1, (int64_t) kv_len), (int64_t) 0); }
 // Keys of page pg in [lo, hi) or below both n_sink and hi.
 __device__ __forceinline__ uint32_t window_mask(int pg, int lo, int hi, int n_sink) {
     return below(hi, pg) & (~below(lo, pg) | below(n_sink, pg));
@@ -150,9 +152,9 @@ __device__ __forceinline__ Item item_of(const Params &p, int b, int qt, int kvh)
     it.n_q = it.bad_rows ? 0 : q1 - q0;
     it.second = it.tok0 + tokens / 2 < it.n_q;
     const int last = min(it.tok0 + tokens, it.n_q) - 1;
-    it.n_keys = it.tok0 < it.n_q ? max(0, min(it.kv_len, it.pos0 + last + 1)) : 0;
+    it.n_keys = it.tok0 < it.n_q ? keys_end((int64_t) it.pos0 + last, it.kv_len) : 0;
     const int end_page = (it.n_keys + kPage - 1) / kPage;
-    it.first = min(window_first(it.pos0 + it.tok0, p.window), it.n_keys);
+    it.first = min(window_first((int64_t) it.pos0 + it.tok0, p.window), it.n_keys);
     it.first_page = it.first == it.n_keys ? end_page : it.first / kPage;
     it.n_sink_pages = min((min(p.n_sink, it.first) + kPage - 1) / kPage, it.first_page);
     it.n_pages = it.n_sink_pages + end_page - it.first_page;
@@ -608,8 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
             if (t == 1 && !I.second) continue;
             const int tq = I.tok0 + t * (kBM / G) + r / G;  // query token index within the sequence
             const int head = I.kvh * G + r % G;
-            const int hi = min(I.kv_len, I.pos0 + tq + 1);  // keys [lo, hi) and sinks below hi are visible
-            const int lo = window_first(I.pos0 + tq, p.window);
+            const int hi = keys_end((int64_t) I.pos0 + tq, I.kv_len);  // keys [lo, hi) and sinks below hi are visible
+            const int lo = window_first((int64_t) I.pos0 + tq, p.window);
             const bool live = tq < I.n_q;
             bool ok = true;
             float m = -INFINITY, l = 0.f;  // the tile's running max (log2 units); this half's row sum

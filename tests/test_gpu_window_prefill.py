@@ -203,3 +203,12 @@ def test_a_nan_key_makes_the_rows_that_see_it_nan(seqs, window, out_dtype, q8):
         o = out[c.starts[i]:c.starts[i + 1]]
         assert torch.equal(o.isnan().all(-1), sees[:, None] & (torch.arange(16, device="cuda") // 4 == 2))
         assert torch.equal(o.isnan().any(-1), o.isnan().all(-1))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_positions_at_the_ends_of_32_bits(q8):
+    """First positions close to 2^31 - 1 (later ones pass it) and below zero (those queries see no key)."""
+    seqs = [(2**31 - 5, 40, 100), (2**31 - 1, 300, 260), (-7, 30, 100), (-(2**31), 3, 10)]
+    c = Chunks(seqs, 8, 2, seed=3, q8=q8)
+    for window, n_sink in ((2**31 - 1, 0), (2**31 - 10, 5), (50, 3)):
+        c.check(c.run(window, n_sink), window, n_sink)
