@@ -141,6 +141,13 @@ void same_device(const at::Tensor &a, const at::Tensor &b) {
 void *ptr(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 size_t bytes(const at::Tensor &t) { return t.defined() ? (size_t) t.nbytes() : 0; }
 
+// A workspace argument: its bytes are its own (an expanded tensor has fewer than it counts).
+at::Tensor space(PyObject *o, const char *what) {
+    at::Tensor t = tensor(o, what);
+    require(!t.defined() || t.is_contiguous(), what);
+    return t;
+}
+
 // An uninitialised tensor on the device of `like`, from torch's allocator (without the dispatcher's
 // way there, which costs as much again).
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like) {
@@ -213,7 +220,7 @@ PyObject *window(PyObject *const *a) {
     const int32_t win = int32(a[7], "window out of range"), sink = int32(a[8], "n_sink out of range");
     const int32_t max_len = int32(a[10], "max_seq_len out of range"), n_ctas = int32(a[16], "n_ctas out of range");
     const float scale = scale_of(a[9]);
-    at::Tensor ws = tensor(a[15], "workspace must be a tensor");
+    at::Tensor ws = space(a[15], "workspace must be a contiguous tensor");
     d.check_devices(c);
     same_device(c.k, ws);
     OnStream s(a[17], c.k.device());
@@ -252,7 +259,7 @@ PyObject *weights(PyObject *const *a) {
     require(acc.size(1) >= max_len, "a row of acc must hold max_seq_len keys (0: every key of a block table)");
     const int32_t n_ctas = int32(a[15], "n_ctas out of range");
     const float scale = scale_of(a[8]);
-    at::Tensor ws = tensor(a[14], "workspace must be a tensor");
+    at::Tensor ws = space(a[14], "workspace must be a contiguous tensor");
     d.check_devices(c);
     same_device(c.k, acc);
     same_device(c.k, ws);
@@ -299,8 +306,8 @@ PyObject *prefill(PyObject *const *a) {
     const int32_t max_q = int32(a[9], "max_q_len out of range"), win = int32(a[10], "window out of range");
     const int32_t sink = int32(a[11], "n_sink out of range"), max_blocks = (int32_t) i[3].size(1);
     const float scale = scale_of(a[12]);
-    at::Tensor out = tensor(a[13], "out must be a tensor"), ws = tensor(a[15], "workspace must be a tensor");
-    at::Tensor sc = tensor(a[16], "scratch must be a tensor");
+    at::Tensor out = tensor(a[13], "out must be a tensor"), ws = space(a[15], "workspace must be a contiguous tensor");
+    at::Tensor sc = space(a[16], "scratch must be a contiguous tensor");
     at::ScalarType type = at::kFloat;
     if (out.defined())
         require(is_out_type(out.scalar_type()) && out.sizes() == q.sizes() && out.is_contiguous(),

@@ -164,6 +164,8 @@ def test_python_checks():
         lambda: L.attn_decode_weights(kc, kc, q, bt, lens, torch.zeros(64).expand(2, 64)),
         lambda: L.attn_prefill_window(kc, kc, q, lens, lens, lens, bt, 1, 5),
         lambda: L.attn_prefill_window(kc, kc, q.transpose(0, 1), torch.zeros(3, dtype=torch.int32), lens, lens, bt, 1, 5),
+        lambda: L.attn_prefill_window(kc, kc, q, torch.zeros(3, dtype=torch.int32), lens, lens, bt, 1, 5,
+                                      workspace=torch.zeros(1, dtype=torch.uint8).expand(1 << 20)),
         lambda: L.Q8Cache.from_planes(torch.zeros(33, 2, 128, dtype=torch.int8), torch.zeros(33, 2, 4).half()),
         lambda: L.Q8Cache.from_planes(torch.zeros(32, 2, 128, dtype=torch.int8), torch.zeros(32, 2, 3).half()),
         lambda: L.KvWeights.from_tensors(acc, torch.zeros(2, 63, dtype=torch.int32), lens, lens),
