@@ -495,6 +495,7 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
     c.lse_out = p.lse_out;
     c.out_bf16 = p.out_bf16;
     c.early = mode == decode::kWeights;
+    c.sparse = mode != decode::kPlain;
     c.mailboxes = ex ? ex->mailboxes : nullptr;
     c.rank = ex ? ex->rank : 0;
     c.n_ranks = ex ? ex->n_ranks : 1;

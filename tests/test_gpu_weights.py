@@ -180,3 +180,18 @@ def test_a_nan_key_makes_its_rows_nan(lens, q8):
         assert acc[i, :n].isnan().all() and torch.equal(acc[i, n:], before[i, n:])
     out[:-1, group] = 0
     assert not out.isnan().any() and not acc[-1].isnan().any()
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(16, 8), (32, 4), (12, 12)])
+@pytest.mark.parametrize("q8", [False, True])
+def test_one_sequence_in_a_long_table(Hq, Hkv, q8):
+    """Fewer pages than CTAs: some CTAs have none, and what earlier calls left in the workspace stays out."""
+    ws = L.WeightsWorkspace(1, Hq, Hkv, 12800 + 4800)
+    ws.buf.fill_(0xff)  # NaN
+    for n in (1, 32, 33, 64, 65, 100, 513, 1000, 2047, 2400, 4700, 0, 40):
+        b = Batch([n], Hq, Hkv, seed=n, q8=q8)
+        b.bt = torch.cat([b.bt, b.bt[:, :1].expand(1, 400)], 1)
+        acc = _acc(b)
+        before = acc.clone()
+        out, lse = _run(b, acc, workspace=ws)
+        _check(b, out, lse, acc, before)

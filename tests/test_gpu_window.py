@@ -279,3 +279,17 @@ def test_a_nan_key_makes_the_rows_that_see_it_nan(lens, out_dtype, q8):
     if not q8:
         out, lse = _run(b, 100000, 4, out_dtype=out_dtype)
         assert out.isnan().all() and lse.isnan().all()
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(16, 8), (32, 4), (12, 12)])
+@pytest.mark.parametrize("q8", [False, True])
+def test_one_sequence_in_a_long_table(Hq, Hkv, q8):
+    """Fewer pages than CTAs: some CTAs have none, and what earlier calls left in the workspace stays out."""
+    ws = L.DecodeWorkspace(1, Hq, Hkv)
+    ws.buf.fill_(0xff)  # NaN
+    for n in (1, 32, 33, 64, 65, 100, 513, 1000, 2047, 2400, 4700, 0, 40):
+        b = Batch([n], Hq, Hkv, seed=n, q8=q8)
+        b.bt = torch.cat([b.bt, b.bt[:, :1].expand(1, 400)], 1)
+        for window, n_sink, dtype in ((1 << 20, 0, torch.float32), (1024, 4, torch.bfloat16), (31, 1, torch.float32)):
+            out, lse = _run(b, window, n_sink, out_dtype=dtype, workspace=ws)
+            _check(b, out, lse, window, n_sink)
