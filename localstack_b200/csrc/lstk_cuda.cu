@@ -39,7 +39,7 @@ struct DeviceInfo {
     size_t decode_q8_smem = 0;
     size_t decode_mode_smem[2][3] = {};  // per [q8_0][mode] (windowed, with accumulated weights)
     size_t prefill_smem = 0;
-    size_t prefill_window_smem[3] = {};  // f32 output, bf16 output, split along the keys
+    size_t prefill_window_smem[5] = {};  // f32 output, bf16 output, the two for many sequences, split along the keys
     size_t append_smem[8] = {};  // per kv_append instantiation (append_kernel)
     size_t gemm_smem = 0;
     size_t evict_smem[2] = {};  // per select_kernel instantiation (one CTA per row, a cluster)
@@ -1062,10 +1062,13 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
     cfg.gridDim = dim3((unsigned) grid);
     if (pw) {
         const bool out16 = pw->out_dtype == LSTK_DTYPE_BF16;
-        const auto kernel = p.n_split > 1 ? prefill_window::prefill_window_kernel<false, true>
-                            : out16       ? prefill_window::prefill_window_kernel<true, false>
-                                          : prefill_window::prefill_window_kernel<false, false>;
-        if ((rc = ensure_smem(&dev->prefill_window_smem[p.n_split > 1 ? 2 : out16], kernel, prefill_window::kSmemBytes,
+        const bool many = n_seqs > prefill_window::kSorted && p.n_qt > 1;  // (never split: an item each at least)
+        const auto kernel = p.n_split > 1   ? prefill_window::prefill_window_kernel<false, true, false>
+                            : many && out16 ? prefill_window::prefill_window_kernel<true, false, true>
+                            : many          ? prefill_window::prefill_window_kernel<false, false, true>
+                            : out16         ? prefill_window::prefill_window_kernel<true, false, false>
+                                            : prefill_window::prefill_window_kernel<false, false, false>;
+        if ((rc = ensure_smem(&dev->prefill_window_smem[p.n_split > 1 ? 4 : 2 * many + out16], kernel, prefill_window::kSmemBytes,
                               "cudaFuncSetAttribute(prefill window)")))
             return rc;
         cfg.blockDim = dim3(prefill_window::kThreads);

@@ -83,7 +83,7 @@ constexpr int kWarpTma = 16, kWarpMma0 = 17, kWarpClear = 19;
 constexpr int kThreads = 640;
 constexpr int kTmemCols = 512;
 
-constexpr int kSorted = 128;  // sequences that the schedule sorts (more are taken in their order)
+constexpr int kSorted = 128;  // sequences that the schedule sorts (more are taken in their order, in kSorted groups)
 
 constexpr int kOffQ = 0;
 constexpr int kOffKv = 2 * kTile;
@@ -105,7 +105,7 @@ struct Barriers {
     uint32_t tmem_base;
     int abort;
     float row[2][2][kBM];       // per tile and key half: row maxima, and the row sums at the end
-    int first_pair[kSorted + 1];  // sorted schedule: pairs before each place of the order
+    int first_pair[kSorted + 1];  // schedule: pairs before each place of the order, or before each group of sequences
     uint8_t order[kSorted];       // sequences, the most key tiles per pair first
 };
 static_assert(sizeof(Barriers) <= 3 * 1024, "barrier block over its reserved bytes");
@@ -163,15 +163,25 @@ __device__ __forceinline__ Item item_of(const Params &p, int b, int qt, int kvh)
     return it;
 }
 
+// Pairs of sequence b that have rows; one for bad rows, whose item reports them.
+__device__ __forceinline__ int pairs_of(const Params &p, int b) {
+    const int tokens = 2 * (kBM / p.group), q0 = p.q_seq_start[b], q1 = p.q_seq_start[b + 1];
+    return q0 < 0 || q1 < q0 || q1 > p.total_tokens ? 1 : min((q1 - q0 + tokens - 1) / tokens, p.n_qt);
+}
+
+__device__ __forceinline__ int group_of(const Params &p) { return (p.n_seqs + kSorted - 1) / kSorted; }
+
 // The schedule. Several sequences, up to kSorted, are ordered by the key tiles of their last pair, most first, and
 // only the pairs that have rows are numbered: x counts the KV heads of a pair, the pairs of a sequence
 // from the last, the sequences in that order. A CTA takes one item of each round of gridDim.x
 // (index), so the long items are dealt out evenly and the short ones fill the last round.
 // Eight chunks of 450 to 511 tokens behind contexts of up to 16 thousand keys (window 4096): a CTA's
-// longest share is 4 x 33 key tiles dealt in the sequences' own order, 3 x 33 and a short item sorted.
-template <bool kSplit>
+// longest share is 4 x 33 key tiles dealt in the sequences' own order, 3 x 33 and a short item sorted. More
+// sequences keep their order and are numbered in kSorted groups (a prompt of 2048 tokens and 199 single queries: 457 us with
+// the pairs that have no rows numbered too, 114 without); those of a pair at most are taken as they come.
+template <bool kSplit, bool kMany>
 struct Schedule {
-    const int *first_pair;  // shared memory; nullptr: unsorted
+    const int *first_pair;  // shared memory; nullptr: every pair of every sequence
     const uint8_t *order;
     int n_items;
     __device__ __forceinline__ int index(int r) const {
@@ -190,26 +200,45 @@ struct Schedule {
     __device__ __forceinline__ Item whole(const Params &p, int x) const {
         const int kvh = x % p.n_head_kv, y = x / p.n_head_kv;
         if (first_pair == nullptr) return item_of(p, y % p.n_seqs, p.n_qt - 1 - y / p.n_seqs, kvh);
-        int lo = 0, hi = p.n_seqs - 1;  // the last place with first_pair <= y
+        int lo = 0, hi = (kMany ? kSorted : p.n_seqs) - 1;  // the last place with first_pair <= y
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (first_pair[mid] <= y) lo = mid; else hi = mid - 1;
+        }
+        if constexpr (kMany) {
+            int rest = y - first_pair[lo], b = lo * group_of(p), pairs;
+            while (rest >= (pairs = pairs_of(p, b))) rest -= pairs, b++;
+            return item_of(p, b, pairs - 1 - rest, kvh);
         }
         return item_of(p, order[lo], first_pair[lo + 1] - 1 - y, kvh);
     }
 };
 
 // Fills the schedule's shared memory (every thread of the block; cost: scratch of kSorted ints).
-template <bool kSplit>
-__device__ __forceinline__ Schedule<kSplit> make_schedule(const Params &p, int *first_pair, uint8_t *order, int *cost, int *pairs) {
-    if (p.n_seqs == 1 || p.n_seqs > kSorted) return {nullptr, nullptr, p.n_items * (kSplit ? p.n_split : 1)};
-    const int b = threadIdx.x, tokens = 2 * (kBM / p.group);
+template <bool kSplit, bool kMany>
+__device__ __forceinline__ Schedule<kSplit, kMany> make_schedule(const Params &p, int *first_pair, uint8_t *order, int *cost, int *pairs) {
+    if (p.n_seqs == 1 || (!kMany && p.n_seqs > kSorted)) return {nullptr, nullptr, p.n_items * (kSplit ? p.n_split : 1)};
+    const int b = threadIdx.x;
+    if constexpr (kMany) {
+        const int per = group_of(p);
+        if (b < kSorted) {
+            int n = 0;
+            for (int c = b * per; c < min((b + 1) * per, p.n_seqs); c++) n += pairs_of(p, c);
+            pairs[b] = n;
+        }
+        __syncthreads();
+        if (b < kSorted) {
+            int before = 0;
+            for (int c = 0; c < b; c++) before += pairs[c];
+            first_pair[b] = before;
+            if (b == kSorted - 1) first_pair[kSorted] = before + pairs[b];
+        }
+        __syncthreads();
+        return {first_pair, nullptr, first_pair[kSorted] * p.n_head_kv * (kSplit ? p.n_split : 1)};
+    }
     if (b < p.n_seqs) {
-        const int q0 = p.q_seq_start[b], q1 = p.q_seq_start[b + 1];
-        const bool bad = q0 < 0 || q1 < q0 || q1 > p.total_tokens;
-        // bad rows keep one item, which reports them
-        pairs[b] = bad ? 1 : min((q1 - q0 + tokens - 1) / tokens, p.n_qt);
-        cost[b] = bad || pairs[b] == 0 ? 0 : item_of(p, b, pairs[b] - 1, 0).n_tiles;
+        pairs[b] = pairs_of(p, b);
+        cost[b] = pairs[b] == 0 ? 0 : item_of(p, b, pairs[b] - 1, 0).n_tiles;  // 0 for bad rows
     }
     __syncthreads();
     if (b < p.n_seqs) {
@@ -298,8 +327,9 @@ __device__ __forceinline__ float row_max(const float (&sc)[32]) {
 extern __shared__ __align__(1024) uint8_t dyn_smem[];
 
 // kOut16: out is bf16, each f32 result rounded once. kSplit: items are runs of key tiles (Params::n_split),
-// whose results go to part_o and part_lse (kOut16 does not matter).
-template <bool kOut16, bool kSplit>
+// whose results go to part_o and part_lse (kOut16 does not matter). kMany: more than kSorted sequences,
+// some of several pairs (an instantiation of its own: its search costs the others 3 % in registers).
+template <bool kOut16, bool kSplit, bool kMany>
 __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __grid_constant__ CUtensorMap qmap,
                                                                      const __grid_constant__ CUtensorMap kmap,
                                                                      const __grid_constant__ CUtensorMap vmap,
@@ -347,8 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_window_kernel(const __gri
     pdl_wait();
     pdl_launch_dependents();
     const int G = p.group;
-    const Schedule<kSplit> sched = make_schedule<kSplit>(p, bars->first_pair, bars->order, reinterpret_cast<int *>(bars->row[0][0]),
-                                         reinterpret_cast<int *>(bars->row[0][1]));
+    const Schedule<kSplit, kMany> sched = make_schedule<kSplit, kMany>(
+        p, bars->first_pair, bars->order, reinterpret_cast<int *>(bars->row[0][0]), reinterpret_cast<int *>(bars->row[0][1]));
 
     // Every role walks the same items. Barrier phases come from running counts: key tile g of this CTA
     // has K in ring use 2 g and V in use 2 g + 1 (stage use % 5, parity (use / 5) % 2) and is phase g of

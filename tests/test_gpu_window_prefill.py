@@ -212,3 +212,26 @@ def test_positions_at_the_ends_of_32_bits(q8):
     c = Chunks(seqs, 8, 2, seed=3, q8=q8)
     for window, n_sink in ((2**31 - 1, 0), (2**31 - 10, 5), (50, 3)):
         c.check(c.run(window, n_sink), window, n_sink)
+
+
+@pytest.mark.parametrize("n,longest", [(129, 400), (300, 700), (200, 3)])
+@pytest.mark.parametrize("q8", [False, True])
+def test_many_sequences_of_uneven_lengths(n, longest, q8):
+    """More sequences than are sorted, most of one query or none, a few of several pairs, and one whose rows are
+    bad (the others are computed all the same)."""
+    rng = np.random.default_rng(n)
+    seqs = []
+    for i in range(n):
+        t = longest if i % 67 == 31 else int(rng.integers(0, 3))
+        p0 = int(rng.integers(0, 200))
+        seqs.append((p0, t, 0 if i % 29 == 5 else p0 + t))
+    c = Chunks(seqs, 8, 4, seed=9, q8=q8)
+    for window, n_sink in ((33, 4), (500, 0)):
+        c.check(c.run(window, n_sink, out_dtype=torch.bfloat16), window, n_sink)
+    want = c.run(90, 2)
+    a, b = int(c.starts[n - 1]), int(c.starts[n])
+    c.start_t[n] = 1 << 30
+    out = torch.zeros_like(want)
+    with pytest.raises(L.LstkError):
+        c.run(90, 2, out=out)
+    assert torch.equal(out[:a], want[:a]) and not out[a:b].any()
