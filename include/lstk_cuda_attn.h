@@ -198,7 +198,8 @@ int lstk_cuda_attn_decode_window_q8(const lstk_kv_layout *layout, const int8_t *
  * (lstk_cuda_attn_decode_weights_workspace_size, which includes the scores of the step: n_head * 4
  * bytes per key); a sequence longer than max_seq_len reports LSTK_ERR_DEVICE_INDEX and attends to its
  * first max_seq_len keys only. A key whose page id is out of range has no weight. A query row with a NaN
- * among its scores makes its out and lse, and the sequence's weights, NaN. The _q8 form as
+ * among its scores makes its out and lse, and the sequence's weights, NaN. After a wait that ran out
+ * (LSTK_ERR_TIMEOUT) acc is as it was before the call, which can be repeated. The _q8 form as
  * lstk_cuda_attn_decode_window_q8. */
 size_t lstk_cuda_attn_decode_weights_workspace_size(int32_t n_seqs, int32_t n_head, int32_t n_head_kv, int32_t head_dim,
                                                     int32_t max_seq_len);

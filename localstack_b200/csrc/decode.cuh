@@ -83,6 +83,7 @@ struct Params {
     int window = 0, n_sink = 0;     // kWindow
     float *scores = nullptr;        // kWeights: [page-group][score_rows][32]
     int score_rows = 0;             // query rows of a full head group (KV heads x group)
+    uint8_t *done = nullptr;        // kWeights: [kMaxCtas], per CTA of the grid 1, or 0 if one of its waits ran out
 };
 
 // First page-group of CTA c's range: floor(c P / G). Computed in double precision, which is
@@ -663,6 +664,13 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
     // sums the pages of its run of sequences, a block-wide scan (warp shuffles, then the warps'
     // totals) gives each run's start.
     __shared__ int32_t warp_tot[kNThreads / 32];
+    // kWeights: set here in every call, so nothing has to clear it, and taken back where a wait runs out.
+    if (kMode == kWeights && threadIdx.x == 0) p.done[blockIdx.x] = 1;
+    auto ran_out = [&](int site, int detail) {
+        report(p.status, kStatusTimeout, site, detail);
+        *abort_flag = 1;
+        if constexpr (kMode == kWeights) p.done[blockIdx.x] = 0;
+    };
     {
         const int per = (p.n_seqs + kNThreads - 1) / kNThreads;
         const int b0 = threadIdx.x * per;
@@ -710,8 +718,7 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
         if (lane == 0) {
             policy = l2_policy_evict_first();
             if (p.start_flag != nullptr && !flag_wait_bounded(p.start_flag, abort_flag, p.wait_ns)) {
-                report(p.status, kStatusTimeout, kSiteDecodeWaitStart, blockIdx.x);
-                *abort_flag = 1;
+                ran_out(kSiteDecodeWaitStart, blockIdx.x);
                 ok = false;
             }
         }
@@ -746,8 +753,7 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
                     const uint32_t k_use = (uint32_t) (i / kNStages);
                     if (k_use > 0 &&
                         !mbar_wait_bounded(smem_u32(&empty[s]), (k_use - 1) & 1, abort_flag, p.wait_ns)) {
-                        report(p.status, kStatusTimeout, kSiteDecodeWaitEmpty, s);
-                        *abort_flag = 1;
+                        ran_out(kSiteDecodeWaitEmpty, s);
                         ok = false;
                         break;
                     }
@@ -822,8 +828,7 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&full[s]), (uint32_t) (i / kNStages) & 1,
                                                              abort_flag, p.wait_ns))) {
                 if (lane == 0) {
-                    report(p.status, kStatusTimeout, kSiteDecodeWaitFull, s);
-                    *abort_flag = 1;
+                    ran_out(kSiteDecodeWaitFull, s);
                 }
                 break;
             }
@@ -898,8 +903,7 @@ __global__ void __launch_bounds__(SplitCfg<kQ8>::kThreads, kQ8 ? 2 : 1) decode_s
                     n_pieces++;
                     if (!__all_sync(0xffffffffu, ok)) {
                         if (lane == 0) {
-                            report(p.status, kStatusTimeout, kSiteDecodeWaitMerge, hw);
-                            *abort_flag = 1;
+                            ran_out(kSiteDecodeWaitMerge, hw);
                         }
                         break;
                     }
@@ -1443,10 +1447,14 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_rows_kernel
 // kWeights, after the combine: acc[b][i] += sum over the query rows r of 2^(score[r][i] - lse2[r]), the
 // softmax weights of key i, with the rows in a fixed order and one thread per key (no atomics: the
 // same inputs give the same bits). A warp takes one page - lane i its key i - and reads that page's
-// record rows of 128 bytes. Rows without a finite maximum (no keys, or every score -inf) add nothing.
+// record rows of 128 bytes. Rows without a finite maximum (no keys, or every score -inf) add nothing. acc is
+// updated in place, so a call whose split did not finish (a wait ran out: records and lse are in part those of
+// another call) leaves it as it is, and can be repeated.
 struct AccumulateParams {
     int n_seqs, n_head, n_head_kv, group, n_hg, score_rows;
     int max_len;  // keys a row may hold (the split kernel's kv_end and table bound)
+    int split_ctas;
+    const uint8_t *done;  // [kMaxCtas], those of split_ctas
     const int32_t *prefix;
     const int32_t *seq_lens;
     const float *scores;
@@ -1462,11 +1470,20 @@ __global__ void __launch_bounds__(kAccumulateThreads, kAccumulateCtas) weights_a
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int n_pages = p.prefix[p.n_seqs];
+    // Each warp reads the split CTAs' bytes for itself, 16 a lane, in the same round trip as the prefix.
+    static_assert(kMaxCtas == 32 * 16, "one load per lane");
+    const uint4 d = reinterpret_cast<const uint4 *>(p.done)[lane];
+    auto missing = [&](uint32_t w, int first) {  // bytes of w (CTAs first .. first + 3) that are of the grid and zero
+        const int n = p.split_ctas - first;
+        return __vcmpeq4(w, 0u) & (n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+    };
+    const uint32_t undone = missing(d.x, 16 * lane) | missing(d.y, 16 * lane + 4) | missing(d.z, 16 * lane + 8) |
+                            missing(d.w, 16 * lane + 12);
     // this warp's stretch of pages
     const int64_t W = (int64_t) gridDim.x * (kAccumulateThreads / 32);
     const int64_t me = (int64_t) blockIdx.x * (kAccumulateThreads / 32) + (threadIdx.x >> 5);
     const int y0 = (int) (me * n_pages / W), y1 = (int) ((me + 1) * n_pages / W);
-    if (y0 == y1) return;
+    if (y0 == y1 || __any_sync(0xffffffffu, undone != 0)) return;
     int b = 0;
     for (int hi = p.n_seqs; b < hi;) {  // largest b with prefix[b] <= y0: the sequence that holds page y0
         const int mid = (b + hi + 1) >> 1;

@@ -533,8 +533,10 @@ size_t lstk_cuda_attn_decode_workspace_size(int32_t n_seqs, int32_t n_head, int3
 
 static int launch_pdl(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, cudaStream_t s);
 
-// Workspace of lstk_cuda_attn_decode_weights: [decode workspace][lse][score records], each 256-byte
-// aligned. A record holds 32 keys' scores of every query row of a head group, in f32.
+// Workspace of lstk_cuda_attn_decode_weights: [decode workspace][lse][a byte per split CTA][score records],
+// each 256-byte aligned. A record holds 32 keys' scores of every query row of a head group, in f32.
+constexpr size_t kWeightsDoneBytes = decode::kMaxCtas;
+static_assert(kWeightsDoneBytes % 256 == 0, "the score records are 256-byte aligned");
 static size_t weights_ws_lse_bytes(int32_t n_seqs, int32_t n_head) {
     return align_up(sizeof(float) * (size_t) n_seqs * n_head, 256);
 }
@@ -547,7 +549,7 @@ size_t lstk_cuda_attn_decode_weights_workspace_size(int32_t n_seqs, int32_t n_he
     const size_t n_hg = (n_head_kv + decode::kHeadsPerGroup - 1) / decode::kHeadsPerGroup;
     const size_t pages = ((size_t) max_seq_len + decode::kPage - 1) / decode::kPage;
     return align_up(lstk_cuda_attn_decode_workspace_size(n_seqs, n_head, n_head_kv, head_dim), 256) +
-           weights_ws_lse_bytes(n_seqs, n_head) +
+           weights_ws_lse_bytes(n_seqs, n_head) + kWeightsDoneBytes +
            (size_t) n_seqs * pages * n_hg * weights_score_rows(n_head, n_head_kv) * decode::kPage * sizeof(float);
 }
 
@@ -673,7 +675,9 @@ static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const
     if (mode == decode::kWeights) {
         uint8_t *more = ws + align_up(lstk_cuda_attn_decode_workspace_size(n_seqs, n_head, hkv, layout->head_dim), 256);
         if (!lse_out) p.lse_out = reinterpret_cast<float *>(more);  // the accumulation needs it
-        p.scores = reinterpret_cast<float *>(more + weights_ws_lse_bytes(n_seqs, n_head));
+        more += weights_ws_lse_bytes(n_seqs, n_head);
+        p.done = more;
+        p.scores = reinterpret_cast<float *>(more + kWeightsDoneBytes);
     }
 
     const size_t smem = q8 ? decode::split_smem_bytes<true>(n_seqs) : decode::split_smem_bytes<false>(n_seqs);
@@ -700,6 +704,8 @@ static int decode_range(const lstk_kv_layout *layout, const void *k_cache, const
     a.n_hg = n_hg;
     a.score_rows = p.score_rows;
     a.max_len = max_seq_len;
+    a.split_ctas = (int) grid;
+    a.done = p.done;
     a.prefix = p.prefix;
     a.seq_lens = seq_lens;
     a.scores = p.scores;
