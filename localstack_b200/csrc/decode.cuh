@@ -283,7 +283,10 @@ __device__ __forceinline__ void process_page(HeadState &st, uint32_t kbase, uint
     const int li = lane >> 3, lr = lane & 7;
 #pragma unroll
     for (int slab = 0; slab < 2; slab++) {
-        if (view.slab_empty(slab)) continue;
+        if (view.slab_empty(slab)) {
+            if constexpr (kMode == kWindow) continue;
+            break;
+        }
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < 8; kk++) {
@@ -484,7 +487,10 @@ __device__ __forceinline__ void process_page_q8(HeadStateQ8 &st, uint32_t kbase,
     const int g = lane >> 2, t = lane & 3;
     const int li = lane >> 3, lr = lane & 7;
     for (int slab = slab_lo; slab < slab_hi; slab++) {
-        if (view.slab_empty(slab)) continue;
+        if (view.slab_empty(slab)) {
+            if constexpr (kMode == kWindow) continue;
+            break;
+        }
         const int tok0 = slab * 16 + g;
         int sb[4][4];
 #pragma unroll
@@ -986,9 +992,8 @@ struct CombineParams {
     const float *part_lse;
     float *out;
     float *lse_out;
-    int out_bf16;  // out is bf16 (the kernels instantiated for a typed output only)
-    int early;     // kWeights: let the accumulation be scheduled now (it waits for this grid)
-    int sparse;    // kWindow, kWeights: a single sequence with fewer pages than CTAs is guessed too
+    int out_bf16;  // kTyped: out is bf16
+    int early;     // kTyped, kWeights: let the accumulation be scheduled now (it waits for this grid)
     // Exchange across ranks (decode_combine_kernel<true>): the mailboxes of the exchange-merge
     // protocol (exchange.cuh) for n_seqs * n_head rows, this rank, the rank count, the flag-wait
     // bound and the device status.
@@ -1179,10 +1184,12 @@ __device__ __forceinline__ void merge_state(float &m, float &den, float4 &acc, f
 // (max, sum, accumulator) state, merged across lane groups by shuffles and across warps in shared
 // memory. Piece i is split CTA c0 + i; its record is slot 0 of that CTA's pair, except for the
 // first piece when the CTA's range began in an earlier segment (slot 1).
+// kTyped: the combine of kWindow and kWeights (a bf16 or f32 output, fewer pages than CTAs, the accumulation
+// behind it); in kPlain's that code cost a single short sequence 1 % (7.81 -> 7.89 us with the split).
 template <bool kExchange, bool kTyped = false>
 __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(const CombineParams p) {
     pdl_wait();  // the split grid's partials and prefix are complete and visible
-    if (p.early) pdl_launch_dependents();
+    if (kTyped && p.early) pdl_launch_dependents();
     const int S = p.dsplit;
     const int b = blockIdx.x, hg = blockIdx.y;
     const int zr = blockIdx.z / S, q = blockIdx.z - zr * S;
@@ -1255,7 +1262,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
     // assumption that head group hg's segment is exactly CTAs [hg g, (hg + 1) g), g = grid / n_hg.
     // That holds when the sequence has at least g pages (P >= grid: CTA hg g's range then starts
     // at the segment's first page-group and no range is empty, so every piece is its CTA's
-    // first, slot 0). With fewer pages the ranges are the same and some are empty: with p.sparse those
+    // first, slot 0). With fewer pages the ranges are the same and some are empty: with kTyped those
     // pieces are dropped once the prefix is there (one sequence of 8000 keys, window 1024: 10.2 -> 9.0 us
     // with the split), otherwise the pieces are loaded again below.
     const int per_hg = p.grid / p.n_hg;
@@ -1274,7 +1281,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
         if (!(guess && P >= p.grid)) {
             if (np == 0) {
                 mode = 1;
-            } else if (guess && p.sparse && np > 1) {
+            } else if (kTyped && guess && np > 1) {
                 mode = 4, n_pc = np;
             } else {
                 const int64_t x0 = (int64_t) p.n_hg * pb + (int64_t) hg * np;
@@ -1301,8 +1308,8 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
             load(i0, c0, n_pc, first_slot, may_be_empty, P);
             accumulate();
         }
-    } else if (mode == 0 || mode == 4) {
-        if (mode == 4) {
+    } else if (mode == 0 || (kTyped && mode == 4)) {
+        if (kTyped && mode == 4) {
             // CTA i of the segment has pages [floor(i np / g), floor((i + 1) np / g)): none if the remainder of
             // i np / g does not reach g with np more. Its record is of another call.
             const int np = plan_s[2];
@@ -1359,7 +1366,7 @@ __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_kernel(cons
 template <bool kTyped>
 __global__ void __launch_bounds__(kCombineThreads, 2) decode_combine_rows_kernel(const CombineParams p) {
     pdl_wait();  // the split grid's partials and prefix are complete and visible
-    if (p.early) pdl_launch_dependents();
+    if (kTyped && p.early) pdl_launch_dependents();
     const int b = blockIdx.x, hg = blockIdx.y, w = blockIdx.z;
     const int kvh = hg * kHeadsPerGroup + w;
     if (kvh >= p.n_head_kv) return;

@@ -495,7 +495,6 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
     c.lse_out = p.lse_out;
     c.out_bf16 = p.out_bf16;
     c.early = mode == decode::kWeights;
-    c.sparse = mode != decode::kPlain;
     c.mailboxes = ex ? ex->mailboxes : nullptr;
     c.rank = ex ? ex->rank : 0;
     c.n_ranks = ex ? ex->n_ranks : 1;
@@ -507,8 +506,8 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
     if (!ex && decode::combine_by_rows(p.n_seqs, p.n_hg, grid)) {
         cfg.gridDim = dim3((unsigned) p.n_seqs, (unsigned) p.n_hg, decode::kHeadsPerGroup);
         return launch_pdl_check(cudaLaunchKernelEx(&cfg,
-                                                   p.out_bf16 ? decode::decode_combine_rows_kernel<true>
-                                                              : decode::decode_combine_rows_kernel<false>,
+                                                   mode != decode::kPlain ? decode::decode_combine_rows_kernel<true>
+                                                                          : decode::decode_combine_rows_kernel<false>,
                                                    c),
                                 "decode_combine_rows_kernel");
     }
@@ -517,8 +516,8 @@ static int launch_decode(const CUtensorMap &kmap, const CUtensorMap &vmap, const
         return launch_pdl_check(cudaLaunchKernelEx(&cfg, decode::decode_combine_kernel<true>, c),
                                 "decode_combine_kernel (exchange)");
     return launch_pdl_check(cudaLaunchKernelEx(&cfg,
-                                               p.out_bf16 ? decode::decode_combine_kernel<false, true>
-                                                          : decode::decode_combine_kernel<false, false>,
+                                               mode != decode::kPlain ? decode::decode_combine_kernel<false, true>
+                                                                      : decode::decode_combine_kernel<false, false>,
                                                c),
                             "decode_combine_kernel");
 }
