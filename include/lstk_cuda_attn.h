@@ -289,7 +289,11 @@ int lstk_cuda_kv_release(const lstk_kv_pages *state, int32_t slot, int32_t keep,
  * the budget would be dropped).
  * The kept keys are then in no particular order, which decode attention does not see; a window
  * (lstk_cuda_attn_decode_window) is taken over positions and does not apply to such a row. Set the
- * row of a removed sequence back to zero (acc, held, shift) before its slot is used again. */
+ * row of a removed sequence back to zero (acc, held, shift) before its slot is used again.
+ * lstk_cuda_kv_release(slot, keep) with keep > 0 knows nothing of this state: keep must be at least
+ * held[slot] (the keys below it are in no order of tokens, so a cut among them drops arbitrary ones), and
+ * acc[slot][keep] onward must then be set to zero, or tokens appended later start with the weights of
+ * those that went. */
 typedef struct lstk_kv_weights {
     float *acc;
     int32_t *pos;

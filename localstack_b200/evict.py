@@ -8,11 +8,15 @@ and when rows have grown past their budget drops the keys with the smallest sums
     for k, v in layers: kv_move(k, v, pages.block_tables, moves)        # their K and V rows
     weights.finish(pages, moves)                                        # lengths, blocks, acc, positions
 
+A sequence is removed, or its newest tokens are taken back, by weights.release(pages, slot, keep):
+DevicePages.release alone leaves the row's weights and positions to the tokens that come after.
+
 The reference has no counterpart: its cache is full when its cells are used up
 (src/kv_cache.cpp:59-83).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 
@@ -109,6 +113,26 @@ class KvWeights:
         self.acc[slot].zero_()
         self.held[slot].zero_()
         self.shift[slot].zero_()
+
+    def release(self, pages, slot, keep=0, stream=None):
+        """pages.release(slot, keep) together with the row: keep <= 0 removes the sequence and clears the row;
+        else the first `keep` keys stay and the weights behind them are cleared (a token appended there later
+        would start with another token's weight).
+
+        The keys below held[slot] are in no order of tokens, so a cut among them would drop arbitrary ones:
+        ValueError, nothing changed (remove the sequence instead). For keep > 0 held[slot] is read back, which
+        waits for the stream: such a call cannot be captured into a graph."""
+        slot, keep = int(slot), int(keep)
+        if not 0 <= slot < self.n_rows:
+            raise ValueError("slot out of range")
+        with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
+            if keep > 0 and keep < int(self.held[slot]):
+                raise ValueError("keep is below held: the row's keys are not in token order there")
+            pages.release(slot, keep, stream)
+            if keep > 0:
+                self.acc[slot, keep:].zero_()
+            else:
+                self.reset(slot)
 
 
 def kv_move(k_cache, v_cache, block_tables, moves: KvMoves, stream=None):
