@@ -99,6 +99,8 @@ class KvWeights:
         if any(t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.device
                for t in (moves.n, moves.src, moves.dst)):
             raise ValueError("moves must be contiguous int32 tensors on the weights' device")
+        if pages.device != self.device:
+            raise ValueError("pages and weights must be on one device")
         check(lib().lstk_cuda_kv_evict_finish(ctypes.byref(pages.state), ctypes.byref(self.state), moves.budget,
                                               _p(moves.n), _p(moves.src), _p(moves.dst), moves.src.shape[1],
                                               _stream(stream, self.device)))
@@ -125,6 +127,8 @@ class KvWeights:
         slot, keep = int(slot), int(keep)
         if not 0 <= slot < self.n_rows:
             raise ValueError("slot out of range")
+        if pages.device != self.device:
+            raise ValueError("pages and weights must be on one device")
         with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
             if keep > 0 and keep < int(self.held[slot]):
                 raise ValueError("keep is below held: the row's keys are not in token order there")

@@ -1,12 +1,13 @@
 """KvWeights.release refuses what would leave the row's weights and positions to other tokens (no GPU)."""
 import pytest
+import torch
 
 import localstack_b200 as L
 
 
 class _Pages:
-    def __init__(self):
-        self.calls = []
+    def __init__(self, device="cpu"):
+        self.calls, self.device = [], torch.device(device)
 
     def release(self, slot, keep, stream=None):
         self.calls.append((slot, keep))
