@@ -10,7 +10,9 @@
 // Every function returns the entry point's status first (the Python side raises LstkError for it)
 // and raises ValueError for tensors that do not fit. Outputs and scratch are allocated on the stream that
 // the kernels run on, so a call on another stream than the current one takes no memory that work
-// on the current one may still use; the current device is left as it was.
+// on the current one may still use; the current device is left as it was. The C call itself runs
+// without the interpreter lock, as one through ctypes does: a launch waits while the stream's queue
+// is full, and the first call loads the kernels.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -134,6 +136,14 @@ struct OnStream {
     }
 };
 
+// Other Python threads may run while the object lives; nothing of Python may be touched meanwhile.
+struct Unlocked {
+    PyThreadState *state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+    Unlocked() = default;
+    Unlocked(const Unlocked &) = delete;
+};
+
 void same_device(const at::Tensor &a, const at::Tensor &b) {
     require(!b.defined() || a.device() == b.device(), "the tensors must be on one device");
 }
@@ -228,18 +238,22 @@ PyObject *window(PyObject *const *a) {
     if (d.B == 0) return result(LSTK_OK, d.out, d.lse);
     const size_t need = lstk_cuda_attn_decode_workspace_size(d.B, d.Hq, c.layout.n_head_kv, (int32_t) kD);
     if (bytes(ws) < need) ws = scratch(need, d.q);
-    const int rc =
-        c.q8() ? lstk_cuda_attn_decode_window_q8(&c.layout, static_cast<const int8_t *>(ptr(c.k)), ptr(c.kd),
-                                                 static_cast<const int8_t *>(ptr(c.v)), ptr(c.vd), ptr(d.q), dtype_of(d.q),
-                                                 d.B, d.Hq, static_cast<int32_t *>(ptr(d.tables)), d.max_blocks,
-                                                 static_cast<int32_t *>(ptr(d.lens)), max_len, win, sink, scale, ptr(d.out),
-                                                 dtype_of(d.out), static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws),
-                                                 n_ctas, s.handle)
-               : lstk_cuda_attn_decode_window(&c.layout, ptr(c.k), ptr(c.v), ptr(d.q), dtype_of(d.q), d.B, d.Hq,
-                                              static_cast<int32_t *>(ptr(d.tables)), d.max_blocks,
-                                              static_cast<int32_t *>(ptr(d.lens)), max_len, win, sink, scale, ptr(d.out),
-                                              dtype_of(d.out), static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws), n_ctas,
-                                              s.handle);
+    int rc;
+    {
+        const Unlocked u;
+        rc = c.q8()
+                 ? lstk_cuda_attn_decode_window_q8(&c.layout, static_cast<const int8_t *>(ptr(c.k)), ptr(c.kd),
+                                                     static_cast<const int8_t *>(ptr(c.v)), ptr(c.vd), ptr(d.q), dtype_of(d.q),
+                                                     d.B, d.Hq, static_cast<int32_t *>(ptr(d.tables)), d.max_blocks,
+                                                     static_cast<int32_t *>(ptr(d.lens)), max_len, win, sink, scale, ptr(d.out),
+                                                     dtype_of(d.out), static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws),
+                                                     n_ctas, s.handle)
+                   : lstk_cuda_attn_decode_window(&c.layout, ptr(c.k), ptr(c.v), ptr(d.q), dtype_of(d.q), d.B, d.Hq,
+                                                  static_cast<int32_t *>(ptr(d.tables)), d.max_blocks,
+                                                  static_cast<int32_t *>(ptr(d.lens)), max_len, win, sink, scale, ptr(d.out),
+                                                  dtype_of(d.out), static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws), n_ctas,
+                                                  s.handle);
+    }
     return result(rc, d.out, d.lse);
 }
 
@@ -270,18 +284,22 @@ PyObject *weights(PyObject *const *a) {
         ws = scratch(lstk_cuda_attn_decode_weights_workspace_size(d.B, d.Hq, c.layout.n_head_kv, (int32_t) kD, (int32_t) max_len),
                      d.q);
     const int64_t stride = d.B > 1 ? acc.stride(0) : acc.size(1);
-    const int rc =
-        c.q8() ? lstk_cuda_attn_decode_weights_q8(&c.layout, static_cast<const int8_t *>(ptr(c.k)), ptr(c.kd),
-                                                  static_cast<const int8_t *>(ptr(c.v)), ptr(c.vd), ptr(d.q),
-                                                  dtype_of(d.q), d.B, d.Hq, static_cast<int32_t *>(ptr(d.tables)),
-                                                  d.max_blocks, static_cast<int32_t *>(ptr(d.lens)), (int32_t) max_len,
-                                                  scale, static_cast<float *>(ptr(acc)), stride, ptr(d.out), dtype_of(d.out),
-                                                  static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws), n_ctas, s.handle)
-               : lstk_cuda_attn_decode_weights(&c.layout, ptr(c.k), ptr(c.v), ptr(d.q), dtype_of(d.q), d.B, d.Hq,
-                                               static_cast<int32_t *>(ptr(d.tables)), d.max_blocks,
-                                               static_cast<int32_t *>(ptr(d.lens)), (int32_t) max_len, scale,
-                                               static_cast<float *>(ptr(acc)), stride, ptr(d.out), dtype_of(d.out),
-                                               static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws), n_ctas, s.handle);
+    int rc;
+    {
+        const Unlocked u;
+        rc = c.q8()
+                 ? lstk_cuda_attn_decode_weights_q8(&c.layout, static_cast<const int8_t *>(ptr(c.k)), ptr(c.kd),
+                                                      static_cast<const int8_t *>(ptr(c.v)), ptr(c.vd), ptr(d.q),
+                                                      dtype_of(d.q), d.B, d.Hq, static_cast<int32_t *>(ptr(d.tables)),
+                                                      d.max_blocks, static_cast<int32_t *>(ptr(d.lens)), (int32_t) max_len,
+                                                      scale, static_cast<float *>(ptr(acc)), stride, ptr(d.out), dtype_of(d.out),
+                                                      static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws), n_ctas, s.handle)
+                   : lstk_cuda_attn_decode_weights(&c.layout, ptr(c.k), ptr(c.v), ptr(d.q), dtype_of(d.q), d.B, d.Hq,
+                                                   static_cast<int32_t *>(ptr(d.tables)), d.max_blocks,
+                                                   static_cast<int32_t *>(ptr(d.lens)), (int32_t) max_len, scale,
+                                                   static_cast<float *>(ptr(acc)), stride, ptr(d.out), dtype_of(d.out),
+                                                   static_cast<float *>(ptr(d.lse)), ptr(ws), bytes(ws), n_ctas, s.handle);
+    }
     return result(rc, d.out, d.lse);
 }
 
@@ -328,19 +346,21 @@ PyObject *prefill(PyObject *const *a) {
     }
     const int32_t *start = static_cast<int32_t *>(ptr(i[0])), *pos0 = static_cast<int32_t *>(ptr(i[1]));
     const int32_t *lens = static_cast<int32_t *>(ptr(i[2])), *tables = static_cast<int32_t *>(ptr(i[3]));
-    int rc;
     if (c.q8()) {
         const size_t room = lstk_cuda_q8_prefill_scratch_size((int32_t) B, max_blocks, hkv);
         if (bytes(sc) < room) sc = scratch(room, q);
-        rc = lstk_cuda_attn_prefill_window_q8(&c.layout, static_cast<const int8_t *>(ptr(c.k)), ptr(c.kd),
-                                              static_cast<const int8_t *>(ptr(c.v)), ptr(c.vd), ptr(q), dtype_of(q),
-                                              (int32_t) B, Hq, start, max_q, q.size(0), pos0, lens, tables, max_blocks, win,
-                                              sink, scale, ptr(out), dtype_of(out), ptr(ws), bytes(ws), ptr(sc), bytes(sc),
-                                              s.handle);
-    } else {
-        rc = lstk_cuda_attn_prefill_window(&c.layout, ptr(c.k), ptr(c.v), ptr(q), dtype_of(q), (int32_t) B, Hq, start, max_q,
-                                           q.size(0), pos0, lens, tables, max_blocks, win, sink, scale, ptr(out),
-                                           dtype_of(out), ptr(ws), bytes(ws), s.handle);
+    }
+    int rc;
+    {
+        const Unlocked u;
+        rc = c.q8() ? lstk_cuda_attn_prefill_window_q8(&c.layout, static_cast<const int8_t *>(ptr(c.k)), ptr(c.kd),
+                                                       static_cast<const int8_t *>(ptr(c.v)), ptr(c.vd), ptr(q),
+                                                       dtype_of(q), (int32_t) B, Hq, start, max_q, q.size(0), pos0, lens,
+                                                       tables, max_blocks, win, sink, scale, ptr(out), dtype_of(out),
+                                                       ptr(ws), bytes(ws), ptr(sc), bytes(sc), s.handle)
+                    : lstk_cuda_attn_prefill_window(&c.layout, ptr(c.k), ptr(c.v), ptr(q), dtype_of(q), (int32_t) B, Hq,
+                                                    start, max_q, q.size(0), pos0, lens, tables, max_blocks, win, sink,
+                                                    scale, ptr(out), dtype_of(out), ptr(ws), bytes(ws), s.handle);
     }
     return result(rc, out);
 }
@@ -378,9 +398,13 @@ PyObject *select(PyObject *const *a) {
     const lstk_kv_weights w = {static_cast<float *>(ptr(acc)), static_cast<int32_t *>(ptr(pos)),
                                static_cast<int32_t *>(ptr(held)), static_cast<int32_t *>(ptr(shift)), (int32_t) rows,
                                (int32_t) cells};
-    const int rc = lstk_cuda_kv_evict_select(&w, static_cast<int32_t *>(ptr(lens)), budget, sink, recent,
-                                             (int32_t) src.size(1), static_cast<int32_t *>(ptr(n)),
-                                             static_cast<int32_t *>(ptr(src)), static_cast<int32_t *>(ptr(dst)), s.handle);
+    int rc;
+    {
+        const Unlocked u;
+        rc = lstk_cuda_kv_evict_select(&w, static_cast<int32_t *>(ptr(lens)), budget, sink, recent, (int32_t) src.size(1),
+                                       static_cast<int32_t *>(ptr(n)), static_cast<int32_t *>(ptr(src)),
+                                       static_cast<int32_t *>(ptr(dst)), s.handle);
+    }
     return result(rc, n, src, dst);
 }
 
@@ -400,10 +424,14 @@ PyObject *move(PyObject *const *a) {
     const int32_t rows = (int32_t) src.size(0), cap = (int32_t) src.size(1), max_blocks = (int32_t) tables.size(1);
     const int32_t *bt = static_cast<int32_t *>(ptr(tables)), *np = static_cast<int32_t *>(ptr(n));
     const int32_t *sp = static_cast<int32_t *>(ptr(src)), *dp = static_cast<int32_t *>(ptr(dst));
-    const int rc = c.q8() ? lstk_cuda_kv_move_q8(&c.layout, static_cast<int8_t *>(ptr(c.k)), ptr(c.kd),
-                                                 static_cast<int8_t *>(ptr(c.v)), ptr(c.vd), bt, rows, max_blocks, np, sp, dp,
-                                                 cap, s.handle)
-                          : lstk_cuda_kv_move(&c.layout, ptr(c.k), ptr(c.v), bt, rows, max_blocks, np, sp, dp, cap, s.handle);
+    int rc;
+    {
+        const Unlocked u;
+        rc = c.q8() ? lstk_cuda_kv_move_q8(&c.layout, static_cast<int8_t *>(ptr(c.k)), ptr(c.kd),
+                                           static_cast<int8_t *>(ptr(c.v)), ptr(c.vd), bt, rows, max_blocks, np, sp, dp, cap,
+                                           s.handle)
+                    : lstk_cuda_kv_move(&c.layout, ptr(c.k), ptr(c.v), bt, rows, max_blocks, np, sp, dp, cap, s.handle);
+    }
     return result(rc);
 }
 
