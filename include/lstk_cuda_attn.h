@@ -285,6 +285,10 @@ int lstk_cuda_kv_release(const lstk_kv_pages *state, int32_t slot, int32_t keep,
  *   3. lstk_cuda_kv_evict_finish: moves acc and pos, clears acc behind the budget, advances held and
  *      shift, and truncates the rows to budget (KvCache::truncate_seq in row order,
  *      src/kv_cache.cpp:85-132: their blocks return to the free stack).
+ * Prefills add nothing to acc: the keys of a prompt are at zero until later queries attend to them, and
+ * step 1 ranks equal keys by index alone. To weigh a prompt before it is cut, pass its last queries to
+ * lstk_cuda_attn_decode_weights as sequences of their own over the same pages (block table row repeated,
+ * seq_lens = position + 1, a row of acc each) and add those rows to the slot's.
  * Between 1 and 3 no token is appended to a row (the moves name the keys that select saw; a later one past
  * the budget would be dropped).
  * The kept keys are then in no particular order, which decode attention does not see; a window

@@ -8,6 +8,14 @@ and when rows have grown past their budget drops the keys with the smallest sums
     for k, v in layers: kv_move(k, v, pages.block_tables, moves)        # their K and V rows
     weights.finish(pages, moves)                                        # lengths, blocks, acc, positions
 
+Only the queries given to attn_decode_weights add up. A prompt's prefill (attn_prefill, attn_prefill_window)
+leaves its keys at zero, and select ranks keys of equal weight by index alone, so a prompt that is to be cut
+needs weights first: give its last R queries to attn_decode_weights as R rows with the slot's block table
+repeated, seq_lens = their positions + 1 and an acc row of zeros each, and add the rows' sum to the slot's acc:
+
+    attn_decode_weights(k, v, q[-R:], table.expand(R, -1).contiguous(), positions + 1, rows)
+    weights.acc[slot, :rows.shape[1]] += rows.sum(0)
+
 A sequence is removed, or its newest tokens are taken back, by weights.release(pages, slot, keep):
 DevicePages.release alone leaves the row's weights and positions to the tokens that come after.
 
