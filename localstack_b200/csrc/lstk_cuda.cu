@@ -978,6 +978,7 @@ size_t lstk_cuda_attn_prefill_window_workspace_size(int32_t n_seqs, int32_t n_he
         cudaGetLastError();
         return plain;
     }
+    max_q_len = (int32_t) std::min<int64_t>(max_q_len, total_tokens);  // as the call does
     const int splits = prefill_window_splits(n_sms, n_seqs, n_head, n_head_kv, max_q_len, max_blocks_per_seq, window, n_sink);
     return align_up(plain, 256) + prefill_window_part_bytes(splits, n_head, total_tokens);
 }
@@ -996,6 +997,7 @@ static int prefill_impl(const lstk_kv_layout *layout, const void *k_cache, const
                             workspace_bytes)))
         return rc;
     const int hkv = layout->n_head_kv, group = n_head / hkv;
+    max_q_len = (int32_t) std::min<int64_t>(max_q_len, total_tokens);  // a bound may be loose; tiles are counted from it
     if (n_seqs == 0 || total_tokens == 0 || max_q_len == 0) return clear_error();
     DeviceInfo *dev = nullptr;
     if ((rc = bind_device(k_cache, &dev))) return rc;
