@@ -56,7 +56,10 @@ thread_local int t_last_device = -1;
 thread_local uint64_t t_pipeline_wait_ns = kWaitLimitNs;
 thread_local const int32_t *t_start_flag = nullptr;
 
+// The message for a failed runtime call. The runtime keeps the error until it is asked for, and the next call's
+// launch_check would report it for launches that succeeded, so it is taken here.
 std::string cuda_msg(const char *what, cudaError_t e) {
+    cudaGetLastError();
     return std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")";
 }
 
