@@ -78,7 +78,8 @@ class DevicePages:
         return self.alloc(slots, None, slots.numel(), cells, positions, ok, stream)
 
     def release(self, slot, keep=0, stream=None):
-        """KvCache::truncate_seq(slot, keep) for keep > 0, remove_seq(slot) otherwise."""
+        """KvCache::truncate_seq(slot, keep) for keep > 0, remove_seq(slot) otherwise (a slot that a KvWeights
+        keeps a row of: KvWeights.release)."""
         check(lib().lstk_cuda_kv_release(ctypes.byref(self.state), int(slot), int(keep),
                                          _stream(stream, self.device)))
 
