@@ -171,10 +171,10 @@ int lstk_cuda_attn_decode_static(const lstk_kv_layout *layout, const void *k_cac
  * the window's first are not looked at. (The window bounds what a step reads, not what a sequence holds:
  * lstk_kv_cache and lstk_kv_pages cannot free pages inside a row, and on release free the row's whole list, so
  * with them a page in between must not go to another sequence. Only a host that keeps tables and free
- * pages of its own can hand it on.) Arguments, results, workspace and limits as lstk_cuda_attn_decode, except: out is f32 or bf16 (out_dtype; bf16, the input
- * type of lstk_cuda_proj, rounds each f32 result once), and lse_out covers the visible keys. A NaN among a
- * row's visible scores makes its out and lse NaN (lstk_cuda_attn_decode leaves out the part of the row that
- * one CTA computed with it). out does not overlap q.
+ * pages of its own can hand it on.) Arguments, results, workspace and limits as lstk_cuda_attn_decode,
+ * except: out is f32 or bf16 (out_dtype; bf16, the input type of lstk_cuda_proj, rounds each f32 result
+ * once), and lse_out covers the visible keys. A NaN among a row's visible scores makes its out and lse NaN
+ * (lstk_cuda_attn_decode leaves out the part of the row that one CTA computed with it). out does not overlap q.
  * max_seq_len bounds seq_lens as there (it sizes the launch only). The _q8 form reads a q8_0 cache
  * with lstk_cuda_attn_decode_q8's semantics, the query's block scale taken as amax * (1 / 127) in f32
  * (a product: its last bit may differ from the quotient's there). */

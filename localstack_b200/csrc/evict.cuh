@@ -457,7 +457,10 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const FinishParams p) 
 }
 
 // KvCache::truncate_seq(row, budget) for the rows over their budget, in row order. One CTA; a warp
-// pushes a row's blocks (its last block first) at the offset that the rows before it leave.
+// pushes a row's blocks (its last block first) at the offset that the rows before it leave. Latency: of
+// lengths, scan, tables and the walk over every slot's blocks for the high-water mark. Together with
+// finish_kernel: 1 row 10 us, 64 rows of 4160 cut to 4096 keys 12 us, 16 rows of 32 k cut to 8 k 32 us, 1024 rows
+// of 300 cut to 256 49 us.
 __global__ void __launch_bounds__(kThreads) truncate_kernel(pages::State st, int budget) {
     __shared__ int warp_sums[32];
     __shared__ int at_s[kThreads];

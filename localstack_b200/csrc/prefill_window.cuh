@@ -21,8 +21,8 @@
 // (256 KiB: the K and V tiles in, Q and K read for S, V for PV). Measured are about 3.7 k cycles: the
 // chain of one tile (S 512-900 as the issuing thread competes with the softmax warps for issue slots,
 // its latency to the softmax 300, max 440, exponentials 1360, P to the last MMA 200, PV's completion
-// 600) is longer than two turns of the exponentials. 8192 tokens, window 4096, 32 / 4 heads: 484 us =
-// 0.53 of the measured bf16 peak, against 528 us with one tile per CTA (prefill.cuh's schedule with the
+// 600) is longer than two turns of the exponentials. 8192 tokens, window 4096, 32 / 4 heads: 490 us =
+// 0.52 of the measured bf16 peak, against 528 us with one tile per CTA (prefill.cuh's schedule with the
 // same masks). Steps that paid, in that measure: turns at the exponentials (623 -> 539 us), P in
 // quarters (-> 526), a warp-uniform issuer (-> 497), f32 exponentials with packed sums (-> 482), sorted
 // sequences (8 chunks behind contexts of up to 16 k: 337 -> 301). Steps that did not: a quarter of the
